@@ -226,6 +226,130 @@ int jh_op_attention_unsplit(const void* q, size_t ldq, const void* k, const void
                             void* out, size_t ldo, const jh_attn_tile* tiles, size_t ntiles,
                             size_t heads, int window, float scale, int wide, void* stream);
 
+/* ------------------------------------------------------------------------
+ * The feed-forward block of models that normalise by the root mean square and
+ * gate their projections: norm -> gated projections -> projection with the
+ * residual's addition, in bf16 or f16 with every gradient, and with e4m3
+ * operands for serving.  No reference counterpart (the reference's encoder has
+ * LayerNorm and runs GEGLU as two kernels, src/cuda/kernels.cu:97-172).
+ *
+ * Element types of these operators, and activations.  e4m3 is OCP FP8 E4M3
+ * (largest magnitude 448), held one byte per value with an f32 scale per row:
+ * the value is code * scale.
+ */
+enum { JH_F32 = 0, JH_BF16 = 1, JH_F16 = 2, JH_E4M3 = 3 };
+enum {
+    JH_ACT_NONE = 0,
+    JH_ACT_RELU = 1,
+    JH_ACT_GELU = 2,       /* z * normal cdf(z)                                  */
+    JH_ACT_GELU_TANH = 3,  /* z/2 * (1 + tanh(sqrt(2/pi) * (z + 0.044715 z^3)))  */
+    JH_ACT_SILU = 4        /* z * sigmoid(z)                                     */
+};
+
+/*
+ * Rules common to them.  Matrices are row-major with a row stride in elements;
+ * pointers and rows lie on 16-byte boundaries (e4m3 rows that rms_norm and
+ * quantize_rows write: 8), row strides are at most 4 MiB.  f32 vectors
+ * (weights of norms, biases, scales, rstd) need 4-byte alignment only.  Feature
+ * counts are multiples of 8, or of 16 where they are the contraction of e4m3
+ * operands; the number of rows is free, 0 included.  An output may not overlap
+ * an input or another output (JH_ERR_INVALID) except where said.  Sums,
+ * statistics and activations are FP32, results are rounded once, and every sum
+ * has a fixed order: the same call gives the same bits.  A row's bits may depend
+ * on the number of rows in the call (kernels are chosen by size).
+ */
+
+/*
+ * s = x + resid (s = x where resid is NULL), rounded to resid's type and stored
+ * to resid_out; out = s / sqrt(mean(s^2) + eps) * w, computed from the rounded
+ * s.  x is f32, bf16 or f16; resid and resid_out are f32 or x's type, and may be
+ * the same memory (NULL together).  hidden is at most 16384; w f32 [hidden].
+ * out is bf16 or f16 (x's type where that is a 16-bit one), or e4m3 with
+ * scales[rows]: scale = max|out| / 448 per row, and each code is the e4m3 value
+ * nearest to the exact quotient of 448 s w by its row's max|s w| (ties to even),
+ * so that codes do not depend on how sums are ordered.  A row of zeros has scale
+ * 0; a NaN gives NaN codes; a row with an infinity has no finite scale.
+ * rstd[rows] (or NULL) receives 1 / sqrt(mean(s^2) + eps) for the backward pass.
+ */
+int jh_op_rms_norm(int x_type, const void* x, size_t ldx, int resid_type, const void* resid, size_t ldr,
+                   void* resid_out, size_t ldro, size_t rows, size_t hidden, const float* w, float eps,
+                   int out_type, void* out, size_t ldo, float* scales, float* rstd, void* stream);
+
+/*
+ * Gradients of jh_op_rms_norm with a 16-bit or f32 output: s is what it stored (or
+ * x without a residual), rstd what it wrote, dy the gradient of out, dres (or
+ * NULL) the gradient that reaches s past the norm.
+ *   g = w dy, n = s rstd:  ds = rstd (g - n mean(g n)) + dres,  dw = sum over rows of dy n.
+ * ds is the gradient of s, thus of x and of resid.  dy is f32, bf16 or f16; s, and
+ * dres with ds, are f32 or dy's type.  ds may be dres, or dy or s where it has
+ * their type and stride.  dw f32 [hidden], or NULL; it needs a workspace of
+ * jh_op_rms_norm_backward_workspace(rows, hidden) bytes, 16-byte aligned.
+ */
+int jh_op_rms_norm_backward(int dy_type, const void* dy, size_t lddy, int s_type, const void* s, size_t lds,
+                            size_t rows, size_t hidden, const float* w, const float* rstd, int ds_type,
+                            const void* dres, size_t lddr, void* ds, size_t ldds, float* dw, void* workspace,
+                            size_t workspace_bytes, void* stream);
+size_t jh_op_rms_norm_backward_workspace(size_t rows, size_t hidden);
+
+/*
+ * q[r] = e4m3 codes of x[r] with scales[r] = max|x[r]| / 448, each code the value
+ * nearest to the exact quotient of 448 x by the row's maximum (ties to even).  x is
+ * f32, bf16 or f16, cols at most 16384.  Quantises activations for, and (once) the
+ * rows of W of, jh_op_linear and jh_op_gated_ffn.
+ */
+int jh_op_quantize_rows(int x_type, const void* x, size_t ldx, size_t rows, size_t cols, void* q, size_t ldq,
+                        float* scales, void* stream);
+
+/*
+ * out = act(z) + resid, z[r, j] = x_scale[r] w_scale[j] sum_k x[r, k] w[j, k] + bias[j].
+ * type (of x and w): bf16, f16 or e4m3.  w [n, k] row-major without padding.
+ * x_scale[rows] and w_scale[n] belong to e4m3 (NULL: ones); bias f32 [n] or NULL.
+ * out and resid (or NULL) have out_type: f32, or type (bf16 for e4m3); resid may
+ * be out itself, with its stride.  pre [rows, n] of type (16-bit types; or NULL)
+ * receives z for the backward pass.
+ */
+int jh_op_linear(int type, const void* x, size_t ldx, const float* x_scale, size_t rows, const void* w,
+                 const float* w_scale, size_t n, size_t k, const float* bias, int act, const void* resid,
+                 size_t ldr, int out_type, void* out, size_t ldo, void* pre, size_t ldp, void* stream);
+
+/*
+ * Gradients of jh_op_linear (bf16 or f16): dz = dy act'(pre), rounded to type;
+ * dx = dz w, dw = dz^T x [n, k] without padding, dbias = column sums of dz before
+ * its rounding, f32 [n].  The gradient of resid is dy.  Each of dx, dw, dbias may
+ * be NULL; x is read for dw, w for dx, pre where act is not JH_ACT_NONE.  dx has
+ * type, dw grad_type (type or f32).  rows = 0 writes zeros to dw and dbias.  The
+ * workspace has jh_op_linear_backward_workspace(rows, n, k, act) bytes (0 where a
+ * size is refused).
+ */
+int jh_op_linear_backward(int type, const void* dy, size_t lddy, const void* x, size_t ldx, size_t rows,
+                          const void* w, size_t n, size_t k, int act, const void* pre, size_t ldp, void* dx,
+                          size_t lddx, int grad_type, void* dw, float* dbias, void* workspace,
+                          size_t workspace_bytes, void* stream);
+size_t jh_op_linear_backward_workspace(size_t rows, size_t n, size_t k, int act);
+
+/*
+ * out = act(x Wg^T) * (x Wu^T) in one kernel: wi [2 inter, k] holds Wg's rows and then
+ * Wu's, as jh_encoder_layer.wi does (JH_EPI_GEGLU_BF16's interleave is not needed).
+ * type as for jh_op_linear, wi_scale [2 inter]; out has type (bf16 for e4m3).  gu
+ * [rows, 2 inter] of type (16-bit types; or NULL) receives both projections for
+ * the backward pass.
+ */
+int jh_op_gated_ffn(int type, const void* x, size_t ldx, const float* x_scale, size_t rows, const void* wi,
+                    const float* wi_scale, size_t inter, size_t k, int act, void* out, size_t ldo, void* gu,
+                    size_t ldgu, void* stream);
+
+/*
+ * Gradients of jh_op_gated_ffn (bf16 or f16): dg = dh u act'(g), du = dh act(g), rounded to
+ * type; dx = [dg du] wi, dwi = [dg du]^T x [2 inter, k] without padding.  dx has type,
+ * dwi grad_type (type or f32); either may be NULL.  The workspace has
+ * jh_op_gated_ffn_backward_workspace(rows, inter, k) bytes (0 where a size is refused).
+ */
+int jh_op_gated_ffn_backward(int type, const void* dh, size_t lddh, const void* gu, size_t ldgu, const void* x,
+                             size_t ldx, size_t rows, const void* wi, size_t inter, size_t k, int act, void* dx,
+                             size_t lddx, int grad_type, void* dwi, void* workspace, size_t workspace_bytes,
+                             void* stream);
+size_t jh_op_gated_ffn_backward_workspace(size_t rows, size_t inter, size_t k);
+
 #ifdef __cplusplus
 }
 #endif

@@ -138,3 +138,129 @@ void launch_final_norm(float* x, int rows, const float* fw, const float* type_em
                        const float* hw, const float* hb, float eps, int hidden, bf16_t* out, hipStream_t stream);
 void launch_gather_f32(const float* src, const int32_t* idx, int rows, int hidden, float* dst, hipStream_t stream);
 void launch_scorer(const float* z, int rows, int hidden, const float* w2, float b2, float* out, hipStream_t stream);
+
+// ---------------------------------------------------------------- linear layers, gated projections, RMS norm
+// (linear*.hip, rms_norm.hip; types and activations are julia1_hip_ops.h's)
+
+// out[q, p] = epilogue(sum over k of Q[q, k] P[p, k]); see linear.hpp for the layouts.
+struct LinearArgs {
+    int type, layout, gated;
+    const void* p;      // W (or, for gradients, W or x by columns)
+    long ldp;
+    const void* q;      // x (or dz)
+    long ldq;
+    int p_cols, q_rows, k;  // output columns (of each half when gated), output rows, contraction length
+    const float* p_scale;   // e4m3: per P row
+    const float* q_scale;   // e4m3: per Q row
+    const float* bias;
+    int act;
+    const void* resid;
+    long ldr;
+    void* out;
+    long ldo;
+    int out_f32;
+    void* pre;          // what the activation is applied to (both halves when gated), or null
+    long ldpre;
+    // set by the launch code
+    float* partial;     // FP32 parts [splits][q_rows][p_cols] instead of the epilogue, or null
+    int splits, split_steps;
+};
+
+// Gradients of a linear layer or of the gated projections (n = both halves' columns there).
+struct LinearGradArgs {
+    int type, gated, act;
+    const void* dy;
+    long lddy;
+    const void* pre;
+    long ldpre;
+    const void* x;
+    long ldx;
+    const void* w;
+    void* dx;
+    long lddx;
+    int grad_f32;
+    void* dw;
+    float* dbias;
+    void* workspace;
+    size_t workspace_bytes;
+};
+
+struct ActGradArgs {
+    const void* dy;
+    long lddy;
+    const void* pre;  // null: dz is dy, only its column sums are wanted
+    long ldpre;
+    void* dz;
+    float* partial;
+    int rows, n, rows_per_block, act;
+};
+
+struct GatedGradArgs {
+    const void* dh;
+    long lddh;
+    const void* gu;
+    long ldgu;
+    void* dgu;
+    int rows, inter, act;
+};
+
+struct RmsNormArgs {
+    int x_type, resid_type, out_type;
+    const void* x;
+    long ldx;
+    const void* resid;
+    long ldr;
+    void* resid_out;
+    long ldro;
+    int rows, hidden;
+    const float* w;
+    float eps;
+    void* out;
+    long ldo;
+    float* scales;
+    float* rstd;
+};
+
+struct RmsNormGradArgs {
+    int dy_type, s_type, ds_type;
+    const void* dy;
+    long lddy;
+    const void* s;
+    long lds;
+    int rows, hidden;
+    const float* w;
+    const float* rstd;
+    const void* dres;
+    long lddr;
+    void* ds;
+    long ldds;
+    float* dw;
+    float* partial;  // [blocks][hidden]
+    int blocks;
+};
+
+// Checked entry points (they throw jh_error before anything is launched).
+void linear_forward(const LinearArgs& a, size_t rows, size_t n, size_t k, int out_type, hipStream_t stream);
+void linear_backward(const LinearGradArgs& a, size_t rows, size_t n, size_t k, hipStream_t stream);
+size_t linear_backward_workspace(size_t rows, size_t n, size_t k, int act, bool gated);
+
+// One kernel each: 128 x 128 tiles, and few rows.
+void launch_linear_tile(const LinearArgs& a, hipStream_t stream);
+void launch_linear_small(const LinearArgs& a, hipStream_t stream);
+
+void rms_norm(const RmsNormArgs& a, hipStream_t stream);
+void quantize_rows(const RmsNormArgs& a, hipStream_t stream);
+void rms_norm_backward(const RmsNormGradArgs& a, size_t workspace_bytes, hipStream_t stream);
+size_t rms_norm_backward_workspace(int rows, int hidden);
+// out[c] = sum over rows of in[r, c], in a fixed order.
+void launch_column_sum(const float* in, int rows, int cols, float* out, hipStream_t stream);
+
+// Argument checks of these operators.  A matrix is 16-byte aligned, its rows too.
+struct Span {
+    uintptr_t at;
+    size_t rows, width, stride;  // bytes
+};
+void check_matrix(const char* op, const char* name, const void* p, size_t ld, size_t rows, size_t cols, int type);
+Span span_of(const void* p, size_t ld, size_t rows, size_t cols, int type);
+bool spans_overlap(const Span& a, const Span& b);
+void check_disjoint(const char* op, const char* out_name, const Span& out, const char* in_name, const Span& in);

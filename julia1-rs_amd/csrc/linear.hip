@@ -1,0 +1,427 @@
+// Linear layers and gated projections: checks, the choice of kernel, the element-wise half of
+// their backward passes and the sums over splits of a contraction.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "linear.hpp"
+
+using namespace lin;
+
+namespace {
+
+constexpr int THREADS = 256;
+
+// act'(z) and act(z) together.
+__device__ inline void act_and_grad(float z, int act, float& value, float& grad) {
+    if (act == JH_ACT_NONE) {
+        value = z;
+        grad = 1.0f;
+    } else if (act == JH_ACT_RELU) {
+        value = z < 0.0f ? 0.0f : z;
+        grad = z > 0.0f ? 1.0f : 0.0f;
+        if (z != z) grad = z;
+    } else if (act == JH_ACT_GELU) {
+        const float cdf = 0.5f * (1.0f + erf_rational(z * 0.70710678118654752f));
+        const float pdf = 0.3989422804014327f * __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z);
+        value = z * cdf;
+        grad = __builtin_fmaf(z, pdf, cdf);
+    } else {
+        const float a = act == JH_ACT_SILU ? 1.0f : kTanhA, b = act == JH_ACT_SILU ? 0.0f : kTanhA * kTanhB;
+        const float zz = z * z, s = sigmoid(z * __builtin_fmaf(b, zz, a));
+        value = z * s;
+        grad = __builtin_fmaf(value * (1.0f - s), __builtin_fmaf(3.0f * b, zz, a), s);
+    }
+}
+
+template <class T>
+__device__ inline void load8_of(const void* p, float (&v)[8]) {
+    const u32x4 r = *(const u32x4*)p;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        v[2 * e] = T::lo(r[e]);
+        v[2 * e + 1] = T::hi(r[e]);
+    }
+}
+
+// dz = dy act'(pre) (rounded to T) and the column sums of its unrounded values, a part per
+// blockIdx.y.  A lane owns 8 columns, the four waves of a workgroup every fourth of its rows;
+// their sums are joined in wave order.
+template <class T>
+__global__ __launch_bounds__(THREADS) void act_grad_kernel(ActGradArgs a) {
+    __shared__ float join[4][64][9];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long c = ((long)blockIdx.x * 64 + lane) * 8;
+    const long r0 = (long)blockIdx.y * a.rows_per_block, r1 = min((long)a.rows, r0 + a.rows_per_block);
+    float sum[8] = {};
+    if (c < a.n) {
+        for (long r = r0 + wave; r < r1; r += 4) {
+            float dz[8];
+            load8_of<T>((const uint16_t*)a.dy + r * a.lddy + c, dz);
+            if (a.pre) {
+                float z[8];
+                load8_of<T>((const uint16_t*)a.pre + r * a.ldpre + c, z);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float v, d;
+                    act_and_grad(z[e], a.act, v, d);
+                    dz[e] *= d;
+                }
+                store16<T>((uint16_t*)a.dz + r * a.n + c, dz);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum[e] += dz[e];
+        }
+    }
+    if (!a.partial) return;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) join[wave][lane][e] = sum[e];
+    __syncthreads();
+    if (wave == 0 && c < a.n) {
+        float* o = a.partial + (long)blockIdx.y * a.n + c;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = ((join[0][lane][e] + join[1][lane][e]) + join[2][lane][e]) + join[3][lane][e];
+    }
+}
+
+// [dg du] = [dh u act'(g), dh act(g)], rounded to T.
+template <class T>
+__global__ __launch_bounds__(THREADS) void gated_grad_kernel(GatedGradArgs a) {
+    const long per = a.inter / 8, i = (long)blockIdx.x * THREADS + threadIdx.x;
+    const long r = i / per, c = (i - r * per) * 8;
+    if (r >= a.rows) return;
+    float dh[8], g[8], u[8], dg[8], du[8];
+    load8_of<T>((const uint16_t*)a.dh + r * a.lddh + c, dh);
+    load8_of<T>((const uint16_t*)a.gu + r * a.ldgu + c, g);
+    load8_of<T>((const uint16_t*)a.gu + r * a.ldgu + a.inter + c, u);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        float v, d;
+        act_and_grad(g[e], a.act, v, d);
+        dg[e] = dh[e] * u[e] * d;
+        du[e] = dh[e] * v;
+    }
+    uint16_t* o = (uint16_t*)a.dgu + r * 2 * a.inter + c;
+    store16<T>(o, dg);
+    store16<T>(o + a.inter, du);
+}
+
+// out[r, c] = sum over s of partial[s][r, c], in split order.
+template <class T>
+__global__ __launch_bounds__(THREADS) void split_sum_kernel(const float* partial, int splits, int rows, int cols,
+                                                            void* out, long ldo, int out_f32) {
+    const long per = cols / 8, i = (long)blockIdx.x * THREADS + threadIdx.x;
+    const long r = i / per, c = (i - r * per) * 8;
+    if (r >= rows) return;
+    const long plane = (long)rows * cols;
+    const float* p = partial + r * cols + c;
+    f32x4 lo = *(const f32x4*)p, hi = *(const f32x4*)(p + 4);
+    for (int s = 1; s < splits; ++s) {
+        lo += *(const f32x4*)(p + s * plane);
+        hi += *(const f32x4*)(p + s * plane + 4);
+    }
+    if (out_f32) {
+        float* o = (float*)out + r * ldo + c;
+        *(f32x4*)o = lo;
+        *(f32x4*)(o + 4) = hi;
+    } else {
+        const float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        store16<T>((uint16_t*)out + r * ldo + c, v);
+    }
+}
+
+unsigned blocks_of(long items, const char* what) {
+    const long b = (items + THREADS - 1) / THREADS;
+    if (b > 0x7fffffffL) throw jh_error(JH_ERR_INVALID, std::string(what) + ": too many elements");
+    return (unsigned)b;
+}
+
+long round_up(long v, long to) { return (v + to - 1) / to * to; }
+
+// ---------------------------------------------------------------- splits of the contraction
+
+long tiles_of(const LinearArgs& a) {
+    const long pw = a.gated ? 64 : 128;
+    return ((a.p_cols + pw - 1) / pw) * ((a.q_rows + 127L) / 128);
+}
+long steps_of(const LinearArgs& a) { return (a.k + STEP_ROWS - 1L) / STEP_ROWS; }
+
+// Into how many parts a gradient product's contraction is cut: as many as the 512 resident
+// workgroups have room for, of eight K steps at least, with the FP32 parts under 16 outputs
+// and 48 MiB.
+constexpr int MAX_SPLITS = 16;
+constexpr long SPLIT_BYTES = 48L << 20;
+int splits_of(const LinearArgs& a) {
+    const long out = (long)a.q_rows * a.p_cols * 4;
+    long s = std::min<long>(MAX_SPLITS, 512 / std::max(1L, tiles_of(a)));
+    s = std::min(s, steps_of(a) / 8);
+    s = std::min(s, SPLIT_BYTES / std::max(1L, out));
+    return (int)std::max(1L, s);
+}
+
+long partial_bytes(const LinearArgs& a) {
+    const int s = splits_of(a);
+    return s > 1 ? round_up((long)s * a.q_rows * a.p_cols * 4, 256) : 0;
+}
+
+template <class T>
+void split_sum(const LinearArgs& a, hipStream_t s) {
+    const unsigned b = blocks_of((long)a.q_rows * (a.p_cols / 8), "linear");
+    JH_LAUNCH(split_sum_kernel<T>, dim3(b), dim3(THREADS), 0, s, a.partial, a.splits, a.q_rows, a.p_cols, a.out, a.ldo,
+              a.out_f32);
+    HIP_CHECK(hipGetLastError());
+}
+
+void run(LinearArgs a, hipStream_t s) {
+    if (a.q_rows == 0) return;
+    a.splits = 1;
+    a.split_steps = 0x7fffffff;
+    if (a.layout == ROWS_ROWS && a.q_rows <= 64) launch_linear_small(a, s);
+    else launch_linear_tile(a, s);
+}
+
+// A gradient product, its contraction split where that fills the GPU.
+void run_gradient(LinearArgs a, float* partial, hipStream_t s) {
+    if (a.q_rows == 0) return;
+    const int splits = splits_of(a);
+    a.split_steps = (int)((steps_of(a) + splits - 1) / splits);
+    a.splits = splits;
+    a.partial = splits > 1 ? partial : nullptr;
+    launch_linear_tile(a, s);
+    if (splits == 1) return;
+    if (a.type == JH_BF16) split_sum<Bf16>(a, s);
+    else split_sum<F16>(a, s);
+}
+
+// ---------------------------------------------------------------- checks
+
+[[noreturn]] void refuse(const char* op, const char* what) {
+    throw jh_error(JH_ERR_INVALID, std::string(op) + ": " + what);
+}
+
+int type_bytes(int type) { return type == JH_F32 ? 4 : type == JH_E4M3 ? 1 : 2; }
+
+}  // namespace
+
+// ---------------------------------------------------------------- shared argument checks
+
+void check_matrix(const char* op, const char* name, const void* p, size_t ld, size_t rows, size_t cols, int type) {
+    const size_t unit = 16 / type_bytes(type);
+    const std::string n = std::string(op) + ": " + name;
+    if (!p) throw jh_error(JH_ERR_INVALID, n + " is null");
+    if ((uintptr_t)p & 15) throw jh_error(JH_ERR_INVALID, n + " is not 16-byte aligned");
+    if (ld < cols && rows > 1) throw jh_error(JH_ERR_INVALID, n + ": row stride below its columns");
+    if (rows > 1 && ld % unit) throw jh_error(JH_ERR_INVALID, n + ": rows are not 16-byte aligned");
+    if (ld > ((size_t)1 << 22) / type_bytes(type)) throw jh_error(JH_ERR_INVALID, n + ": row stride over 4 MiB");
+}
+
+Span span_of(const void* p, size_t ld, size_t rows, size_t cols, int type) {
+    return Span{(uintptr_t)p, p ? rows : 0, cols * type_bytes(type), std::max(ld, cols) * type_bytes(type)};
+}
+
+// Whether two strided matrices share a byte.  With equal row strides their columns are
+// compared within a row (two column ranges of one buffer do not overlap); otherwise their
+// whole extents are.
+bool spans_overlap(const Span& a, const Span& b) {
+    if (!a.rows || !b.rows || !a.width || !b.width) return false;
+    const uintptr_t a1 = a.at + (a.rows - 1) * a.stride + a.width, b1 = b.at + (b.rows - 1) * b.stride + b.width;
+    if (a1 <= b.at || b1 <= a.at) return false;
+    if (a.stride != b.stride || a.rows == 1 || b.rows == 1) return true;
+    const uintptr_t d = (b.at > a.at ? b.at - a.at : a.stride - (a.at - b.at) % a.stride) % a.stride;
+    return d < a.width || d + b.width > a.stride;
+}
+
+void check_disjoint(const char* op, const char* out_name, const Span& out, const char* in_name, const Span& in) {
+    if (spans_overlap(out, in))
+        throw jh_error(JH_ERR_INVALID, std::string(op) + ": " + out_name + " overlaps " + in_name);
+}
+
+// ---------------------------------------------------------------- entry points
+
+namespace {
+
+void check_sizes(const char* op, int type, size_t rows, size_t n, size_t k) {
+    if (type != JH_BF16 && type != JH_F16 && type != JH_E4M3) refuse(op, "type must be bf16, f16 or e4m3");
+    if (n == 0 || k == 0) refuse(op, "empty feature dimension");
+    if (n % 8) refuse(op, "output features must be a multiple of 8");
+    if (k % (type == JH_E4M3 ? 16 : 8)) refuse(op, "input features must be a multiple of 16 bytes");
+    if (rows > ((size_t)1 << 30) || n > ((size_t)1 << 22)) refuse(op, "too large");
+}
+
+void check_act(const char* op, int act) {
+    if (act < JH_ACT_NONE || act > JH_ACT_SILU) refuse(op, "unknown activation");
+}
+
+}  // namespace
+
+void linear_forward(const LinearArgs& a, size_t rows, size_t n, size_t k, int out_type, hipStream_t s) {
+    const char* op = a.gated ? "gated_ffn" : "linear";
+    check_sizes(op, a.type, rows, n, k);
+    check_act(op, a.act);
+    const int half = a.type == JH_E4M3 ? JH_BF16 : a.type;
+    if (out_type != half && (a.gated || out_type != JH_F32))
+        refuse(op, a.gated ? "the output has the operands' type (bf16 for e4m3)"
+                           : "the output has the operands' type (bf16 for e4m3) or f32");
+    if (a.type != JH_E4M3 && (a.p_scale || a.q_scale)) refuse(op, "scales belong to e4m3 operands");
+    if (a.type == JH_E4M3 && a.pre) refuse(op, "pre-activations are kept for 16-bit operands");
+    const size_t w_rows = a.gated ? 2 * n : n;
+    if (rows == 0) return;
+    check_matrix(op, "x", a.q, a.ldq, rows, k, a.type);
+    check_matrix(op, "w", a.p, a.ldp, w_rows, k, a.type);
+    check_matrix(op, "out", a.out, a.ldo, rows, n, out_type);
+    if (a.resid) check_matrix(op, "resid", a.resid, a.ldr, rows, n, out_type);
+    if (a.pre) check_matrix(op, "pre", a.pre, a.ldpre, rows, w_rows, half);
+    // The tiles address both halves of Wi by 31-bit offsets from its first row.
+    if (a.gated && (n + 256) * k * type_bytes(a.type) >= ((size_t)1 << 31)) refuse(op, "w of 4 GiB or more");
+    const Span x = span_of(a.q, a.ldq, rows, k, a.type), w = span_of(a.p, a.ldp, w_rows, k, a.type);
+    const Span out = span_of(a.out, a.ldo, rows, n, out_type), pre = span_of(a.pre, a.ldpre, rows, w_rows, half);
+    const Span resid = span_of(a.resid, a.ldr, rows, n, out_type);
+    check_disjoint(op, "out", out, "x", x);
+    check_disjoint(op, "out", out, "w", w);
+    check_disjoint(op, "pre", pre, "x", x);
+    check_disjoint(op, "pre", pre, "w", w);
+    check_disjoint(op, "pre", pre, "out", out);
+    check_disjoint(op, "pre", pre, "resid", resid);
+    // out may be resid itself: every element is read by the thread that writes it.
+    if (a.resid != a.out || a.ldr != a.ldo) check_disjoint(op, "out", out, "resid", resid);
+    run(a, s);
+}
+
+namespace {
+
+// Workspace of a backward pass: the gradient before the activation, then FP32 parts (of the
+// column sums, and after them of the products: the stream runs one after the other).
+struct BackwardPlan {
+    LinearArgs dx{}, dw{};
+    long dz_bytes = 0, part_bytes = 0;
+    int sum_blocks = 0, rows_per_block = 0;
+    size_t bytes() const { return (size_t)(dz_bytes + part_bytes); }
+};
+
+BackwardPlan plan_backward(int type, size_t rows, size_t n, size_t k, bool keeps_dz, bool sums) {
+    BackwardPlan p;
+    p.dx.type = p.dw.type = type;
+    p.dx.layout = COLS_ROWS;
+    p.dx.p_cols = (int)k;
+    p.dx.q_rows = (int)rows;
+    p.dx.k = (int)n;
+    p.dw.layout = COLS_COLS;
+    p.dw.p_cols = (int)k;
+    p.dw.q_rows = (int)n;
+    p.dw.k = (int)rows;
+    p.dz_bytes = keeps_dz ? round_up((long)rows * n * 2, 256) : 0;
+    p.part_bytes = std::max(partial_bytes(p.dx), partial_bytes(p.dw));
+    if (sums) {
+        const long across = (n + 511) / 512, want = std::max(1L, 1024 / across);
+        p.rows_per_block = (int)std::max(8L, ((long)rows + want - 1) / want);
+        p.sum_blocks = (int)(((long)rows + p.rows_per_block - 1) / p.rows_per_block);
+        p.part_bytes = std::max(p.part_bytes, round_up((long)p.sum_blocks * n * 4, 256));
+    }
+    return p;
+}
+
+void check_workspace(const char* op, const void* ws, size_t bytes, size_t need) {
+    if (need == 0) return;
+    if (!ws || ((uintptr_t)ws & 15)) refuse(op, "needs a 16-byte aligned workspace");
+    if (bytes < need) refuse(op, "workspace too small");
+}
+
+// The two gradient products of a linear layer: dx = dz W and dw = dzᵀ x.
+void run_products(const BackwardPlan& p, const void* dz, long lddz, const LinearGradArgs& a, float* partial,
+                  hipStream_t s) {
+    if (a.dx) {
+        LinearArgs d = p.dx;
+        d.p = a.w;
+        d.ldp = p.dx.p_cols;
+        d.q = dz;
+        d.ldq = lddz;
+        d.out = a.dx;
+        d.ldo = a.lddx;
+        run_gradient(d, partial, s);
+    }
+    if (a.dw) {
+        LinearArgs d = p.dw;
+        d.p = a.x;
+        d.ldp = a.ldx;
+        d.q = dz;
+        d.ldq = lddz;
+        d.out = a.dw;
+        d.ldo = p.dw.p_cols;
+        d.out_f32 = a.grad_f32;
+        run_gradient(d, partial, s);
+    }
+}
+
+}  // namespace
+
+size_t linear_backward_workspace(size_t rows, size_t n, size_t k, int act, bool gated) {
+    const char* op = gated ? "gated_ffn_backward" : "linear_backward";
+    check_sizes(op, JH_BF16, rows, n, k);
+    if (gated && n % 16) refuse(op, "output features must be a multiple of 8");
+    check_act(op, act);
+    return plan_backward(JH_BF16, rows, n, k, gated || act != JH_ACT_NONE, !gated).bytes();
+}
+
+void linear_backward(const LinearGradArgs& a, size_t rows, size_t n, size_t k, hipStream_t s) {
+    const char* op = a.gated ? "gated_ffn_backward" : "linear_backward";
+    if (a.type == JH_E4M3) refuse(op, "gradients are of bf16 or f16 operands");
+    check_sizes(op, a.type, rows, n, k);
+    check_act(op, a.act);
+    const size_t inter = n / 2, dy_cols = a.gated ? inter : n;
+    if (a.gated && n % 16) refuse(op, "output features must be a multiple of 8");
+    const bool keeps_dz = a.gated || a.act != JH_ACT_NONE;
+    const int grad_type = a.grad_f32 ? JH_F32 : a.type;
+    if (!a.dx && !a.dw && !a.dbias) refuse(op, "no gradient asked for");
+    const BackwardPlan p = plan_backward(a.type, rows, n, k, keeps_dz, a.dbias != nullptr);
+    check_workspace(op, a.workspace, a.workspace_bytes, p.bytes());
+    const Span ws = span_of(a.workspace, p.bytes(), p.bytes() ? 1 : 0, p.bytes(), JH_E4M3);
+    if (rows) check_matrix(op, a.gated ? "dh" : "dy", a.dy, a.lddy, rows, dy_cols, a.type);
+    if (rows && keeps_dz) check_matrix(op, a.gated ? "gu" : "pre", a.pre, a.ldpre, rows, n, a.type);
+    if (a.dx && rows) {
+        check_matrix(op, "w", a.w, k, n, k, a.type);
+        check_matrix(op, "dx", a.dx, a.lddx, rows, k, a.type);
+    }
+    if (a.dw) {
+        if (rows) check_matrix(op, "x", a.x, a.ldx, rows, k, a.type);
+        check_matrix(op, "dw", a.dw, k, n, k, grad_type);
+    }
+    const Span in[4] = {span_of(a.dy, a.lddy, rows, dy_cols, a.type),
+                        span_of(keeps_dz ? a.pre : nullptr, a.ldpre, rows, n, a.type),
+                        span_of(a.dw ? a.x : nullptr, a.ldx, rows, k, a.type),
+                        span_of(a.dx ? a.w : nullptr, k, n, k, a.type)};
+    const Span out[4] = {span_of(a.dx, a.lddx, rows, k, a.type), span_of(a.dw, k, n, k, grad_type),
+                         span_of(a.dbias, n, 1, n, JH_F32), ws};
+    for (int o = 0; o < 4; ++o) {
+        for (int i = 0; i < 4; ++i) check_disjoint(op, "an output or the workspace", out[o], "an input", in[i]);
+        for (int i = 0; i < o; ++i) check_disjoint(op, "an output", out[o], "another", out[i]);
+    }
+
+    uint8_t* const base = (uint8_t*)a.workspace;
+    float* const partial = (float*)(base + p.dz_bytes);
+    const void* dz = a.dy;
+    long lddz = a.lddy;
+    if (keeps_dz) {
+        dz = base;
+        lddz = (long)n;
+    }
+    if (a.gated && rows) {
+        const GatedGradArgs g{a.dy, a.lddy, a.pre, a.ldpre, base, (int)rows, (int)inter, a.act};
+        const dim3 grid(blocks_of((long)rows * (inter / 8), op));
+        if (a.type == JH_BF16) JH_LAUNCH(gated_grad_kernel<Bf16>, grid, dim3(THREADS), 0, s, g);
+        else JH_LAUNCH(gated_grad_kernel<F16>, grid, dim3(THREADS), 0, s, g);
+        HIP_CHECK(hipGetLastError());
+    } else if (!a.gated && (keeps_dz || a.dbias)) {
+        // Rows per workgroup are the plan's with the sums, as the parts are stored by them.
+        const BackwardPlan q = plan_backward(a.type, rows, n, k, keeps_dz, true);
+        if (rows) {
+            const ActGradArgs g{a.dy, a.lddy, keeps_dz ? a.pre : nullptr, a.ldpre, base, a.dbias ? partial : nullptr,
+                                (int)rows, (int)n, q.rows_per_block, a.act};
+            const dim3 grid((unsigned)((n + 511) / 512), (unsigned)q.sum_blocks);
+            if (a.type == JH_BF16) JH_LAUNCH(act_grad_kernel<Bf16>, grid, dim3(THREADS), 0, s, g);
+            else JH_LAUNCH(act_grad_kernel<F16>, grid, dim3(THREADS), 0, s, g);
+            HIP_CHECK(hipGetLastError());
+        }
+        if (a.dbias) launch_column_sum(partial, q.sum_blocks, (int)n, a.dbias, s);
+    }
+    run_products(p, dz, lddz, a, partial, s);
+}

@@ -1,0 +1,375 @@
+// Shared by the linear and gated-projection kernels (linear_tile.hip,
+// linear_wide.hip, linear_small.hip): arguments, operand staging into LDS,
+// fragment reads, the MFMA of each type, activations and the epilogue.
+//
+// All of them compute out[q, p] = Σ_k Q[q, k] · P[p, k], P the operand whose index
+// runs along an output row (MFMA's first operand, so a lane ends with runs of
+// consecutive output columns) and Q the one that counts output rows.  Each operand
+// lies in memory either with k contiguous (rows of P or Q, as X and W in X·Wᵀ) or
+// with k as its row index (as W in dX = dZ·W, or dZ and X in dW = dZᵀ·X).
+//
+// A K step covers 128 bytes of every row: 64 elements of 16 bits or 128 of 8.
+#pragma once
+
+#include "../../include/julia1_hip.h"
+#include "../../include/julia1_hip_ops.h"
+#include "kernels.hpp"
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef int32_t i32x8 __attribute__((ext_vector_type(8)));
+typedef f32x4 f32x4_u __attribute__((aligned(4)));  // bias and scales need no more than their type's alignment
+typedef short lin_s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) lin_s16x4 lds_lin_s16x4;
+
+namespace lin {
+
+constexpr int STEP_BYTES = 128;  // of each operand row per K step
+constexpr int STEP_ROWS = 64;    // contraction rows per K step (16-bit types only)
+
+// Operand types.  Frag is what a lane holds of 16 operand rows and one K step: 16 bytes of
+// each half of the step (make); which of them is which k does not matter, as both operands
+// agree.  half is the type of 16-bit outputs.
+struct Bf16 {
+    static constexpr int bytes = 2;
+    struct Frag {
+        bf16x8 v[2];
+    };
+    __device__ static Frag make(u32x4 a, u32x4 b) {
+        return {{__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b)}};
+    }
+    __device__ static f32x4 mfma(const Frag& a, const Frag& b, f32x4 c) {
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[0], b.v[0], c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[1], b.v[1], c, 0, 0, 0);
+    }
+    __device__ static uint32_t pack(float a, float b) { return pack2(a, b); }
+    __device__ static float lo(uint32_t v) { return __builtin_bit_cast(float, v << 16); }
+    __device__ static float hi(uint32_t v) { return __builtin_bit_cast(float, v & 0xffff0000u); }
+};
+
+struct F16 {
+    static constexpr int bytes = 2;
+    struct Frag {
+        f16x8 v[2];
+    };
+    __device__ static Frag make(u32x4 a, u32x4 b) {
+        return {{__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b)}};
+    }
+    __device__ static f32x4 mfma(const Frag& a, const Frag& b, f32x4 c) {
+        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.v[0], b.v[0], c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a.v[1], b.v[1], c, 0, 0, 0);
+    }
+    __device__ static uint32_t pack(float a, float b) {
+        return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)a) |
+               (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)b) << 16;
+    }
+    __device__ static float lo(uint32_t v) { return (float)__builtin_bit_cast(_Float16, (uint16_t)v); }
+    __device__ static float hi(uint32_t v) { return (float)__builtin_bit_cast(_Float16, (uint16_t)(v >> 16)); }
+};
+
+// e4m3 operands for bf16 outputs: one MFMA of K = 128 (block scales 2^0, biased exponent
+// 127), at twice the rate of the 16-bit MFMAs.  The hardware aligns the products of one
+// such MFMA to the largest and drops what lies about 2^-13 below it, whatever the
+// accumulator's 32 bits: against 64 bits the sums are off by 1.5e-5 of their norm (normally
+// distributed operands, K from 16 to 4096), 1/100 of what rounding them to bf16 costs.
+struct E4m3 : Bf16 {
+    static constexpr int bytes = 1;
+    typedef i32x8 Frag;
+    __device__ static Frag make(u32x4 a, u32x4 b) {
+        return i32x8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
+    }
+    __device__ static f32x4 mfma(const Frag& a, const Frag& b, f32x4 c) {
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+    }
+};
+
+// e4m3 operands for FP32 outputs: the codes widened to bf16 (exact) for the bf16 MFMA, whose
+// sums are good to 32 bits.
+struct E4m3Wide : Bf16 {
+    static constexpr int bytes = 1;
+    struct Frag {
+        bf16x8 v[4];
+    };
+    __device__ static bf16x8 widen8(uint32_t a, uint32_t b) {
+        const bf16x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, false);
+        const bf16x2 p1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, true);
+        const bf16x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false);
+        const bf16x2 p3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true);
+        return bf16x8{p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
+    }
+    __device__ static Frag make(u32x4 a, u32x4 b) {
+        return {{widen8(a[0], a[1]), widen8(a[2], a[3]), widen8(b[0], b[1]), widen8(b[2], b[3])}};
+    }
+    __device__ static f32x4 mfma(const Frag& a, const Frag& b, f32x4 c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[i], b.v[i], c, 0, 0, 0);
+        return c;
+    }
+};
+
+// Layouts of (P, Q).
+enum { ROWS_ROWS = 0, COLS_ROWS = 1, COLS_COLS = 2 };  // ROWS: k contiguous; COLS: k is the row index
+enum { EPI_LINEAR = 0, EPI_GATED = 1 };
+
+// ---------------------------------------------------------------- activations
+
+// Sigmoid from the hardware's exponential and reciprocal (1 ulp each).
+__device__ inline float sigmoid(float x) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
+}
+constexpr float kTanhA = 1.5957691216057308f;   // 2 sqrt(2 / pi): gelu_tanh(z) = z sigmoid(A (z + B z^3))
+constexpr float kTanhB = 0.044715f;
+
+// act(v) in place.  relu passes a NaN on, as the others do.
+template <int N>
+__device__ inline void activate(float (&v)[N], int act) {
+    if (act == JH_ACT_NONE) return;
+    if (act == JH_ACT_RELU) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = v[e] < 0.0f ? 0.0f : v[e];
+    } else if (act == JH_ACT_GELU) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = gelu_erf(v[e]);
+    } else {
+        const float a = act == JH_ACT_SILU ? 1.0f : kTanhA, b = act == JH_ACT_SILU ? 0.0f : kTanhA * kTanhB;
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] *= sigmoid(v[e] * __builtin_fmaf(b, v[e] * v[e], a));
+    }
+}
+
+// ---------------------------------------------------------------- operand staging
+
+__device__ constexpr int row_swz(int r) { return (r >> 1) & 7; }
+__device__ constexpr int col_swz(int k) { return ((k & 3) << 1) | (((k >> 3) & 1) << 3); }
+
+// Which P row (output column, counted from the tile's first) LDS row `r` holds, so that a
+// lane's four accumulator tiles of a 64-row block are 16 consecutive columns: row
+// 16i + 4g + e of a block holds column 16g + 4i + e.  EPI_GATED: i < 2 the gate and
+// i >= 2 the up projection of columns 8g + 4(i % 2) + e of the block's 32.
+template <int EPI>
+__device__ inline int p_row(int r, int inter) {
+    const int blk = r >> 6, i = (r >> 4) & 3, g = (r >> 2) & 3, e = r & 3;
+    if constexpr (EPI == EPI_GATED) return blk * 32 + 8 * g + 4 * (i & 1) + e + (i & 2 ? inter : 0);
+    else return blk * 64 + 16 * g + 4 * i + e;
+}
+
+// Out-of-range offset of a buffer load: past every resource's size, so the load writes
+// zeros to LDS.
+constexpr uint32_t OOB = 0x80000000u;
+
+__device__ inline i32x4 bounded_rsrc(const void* base, long bytes) {
+    return make_rsrc(base, (uint64_t)(bytes < 0 ? 0 : bytes < 0x7fffffffL ? bytes : 0x7fffffffL));
+}
+
+__device__ inline void dma16(uint32_t lds, uint32_t voff, i32x4 rsrc, uint32_t soff) {
+    asm volatile("buffer_load_dwordx4 %1, %2, %3 offen lds" ::"{m0}"(lds), "v"(voff), "s"(rsrc), "s"(soff) : "memory");
+}
+
+// ---------------------------------------------------------------- fragments
+
+// k-contiguous operand staged as 128-byte rows, 16-byte chunks XOR-swizzled by the row:
+// the fragment of K half `h` (chunks 4h + g) of row `r`.
+__device__ inline u32x4 row_frag(const uint8_t* part, int r, int h, int g) {
+    return *(const u32x4*)(part + r * 128 + (((h * 4 + g) ^ row_swz(r)) << 4));
+}
+
+// Operand with k as row index, staged as 64 rows of 128 columns (256 bytes): the fragment
+// of columns c0 .. c0+15 and K half `h`, k = 32h + 8g + (0..7), by two transposing reads
+// (in each 16 lanes, lane j addresses row j / 4, columns 4 (j % 4); lane i receives four
+// rows of column i).
+__device__ inline u32x4 col_frag(const uint8_t* part, int c0, int h, int lane) {
+    const int g = lane >> 4, k = h * 32 + g * 8 + ((lane & 15) >> 2), q = (c0 >> 3) + ((lane & 3) >> 1);
+    const uint8_t* p0 = part + k * 256 + ((q ^ col_swz(k)) << 4) + (lane & 1) * 8;
+    const uint8_t* p1 = p0 + 4 * 256;  // col_swz(k + 4) == col_swz(k): k % 8 < 4
+    const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_lin_s16x4*)p0));
+    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_lin_s16x4*)p1));
+    return u32x4{lo[0], lo[1], hi[0], hi[1]};
+}
+
+// The fragment of 16 operand rows (or columns) from `first` of a staged part.
+template <class T, bool COLS>
+__device__ inline typename T::Frag frag(const uint8_t* part, int first, int lane) {
+    if constexpr (COLS) {
+        return T::make(col_frag(part, first, 0, lane), col_frag(part, first, 1, lane));
+    } else {
+        const int r = first + (lane & 15), g = lane >> 4;
+        return T::make(row_frag(part, r, 0, g), row_frag(part, r, 1, g));
+    }
+}
+
+// ---------------------------------------------------------------- epilogue
+
+// Four accumulator tiles whose lane group g holds columns 16i + 4g + e (P staged by
+// columns) -> lane group g holds columns 16g + 4i + e, as P staged by rows leaves them: a
+// 4 x 4 transpose over (tile, lane group) by half-wave and 16-lane swaps.
+__device__ inline void transpose_groups(f32x4 (&t)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        uint32_t r[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float x = t[i][e];  // a bit cast of a vector's element itself would take its first
+            r[i] = __builtin_bit_cast(uint32_t, x);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+            const u32x2 s = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(r[i], r[i + 1], false, false));
+            r[i] = s[0];
+            r[i + 1] = s[1];
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const u32x2 s = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(r[i], r[i + 2], false, false));
+            r[i] = s[0];
+            r[i + 2] = s[1];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[i][e] = __builtin_bit_cast(float, r[i]);
+    }
+}
+
+template <class T, int N>
+__device__ inline void store16(void* dst, const float (&v)[N]) {
+#pragma unroll
+    for (int c = 0; c < N; c += 8)
+        *(u32x4*)((uint16_t*)dst + c) = u32x4{T::pack(v[c], v[c + 1]), T::pack(v[c + 2], v[c + 3]),
+                                              T::pack(v[c + 4], v[c + 5]), T::pack(v[c + 6], v[c + 7])};
+}
+
+// Eight columns of one output row: c0 .. c0+7 (c0 % 8 == 0 and c0 < a.p_cols).
+template <class T>
+__device__ inline void finish8(const LinearArgs& a, float (&z)[8], long t, int c0, float qs) {
+    if constexpr (T::bytes == 1) {
+        if (a.p_scale) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const f32x4 s = *(const f32x4_u*)(a.p_scale + c0 + 4 * h);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) z[4 * h + e] *= qs * s[e];
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) z[e] *= qs;
+        }
+    }
+    if (a.bias) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const f32x4 b = *(const f32x4_u*)(a.bias + c0 + 4 * h);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[4 * h + e] += b[e];
+        }
+    }
+    if constexpr (T::bytes == 2)
+        if (a.pre) store16<T>((uint16_t*)a.pre + t * a.ldpre + c0, z);
+    activate(z, a.act);
+    if (a.out_f32) {
+        float* o = (float*)a.out + t * a.ldo + c0;
+        if (a.resid) {
+            const float* r = (const float*)a.resid + t * a.ldr + c0;
+            const f32x4 r0 = *(const f32x4*)r, r1 = *(const f32x4*)(r + 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                z[e] += r0[e];
+                z[4 + e] += r1[e];
+            }
+        }
+        *(f32x4*)o = f32x4{z[0], z[1], z[2], z[3]};
+        *(f32x4*)(o + 4) = f32x4{z[4], z[5], z[6], z[7]};
+    } else {
+        if (a.resid) {
+            const u32x4 r = *(const u32x4*)((const uint16_t*)a.resid + t * a.ldr + c0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                z[2 * e] += T::lo(r[e]);
+                z[2 * e + 1] += T::hi(r[e]);
+            }
+        }
+        store16<T>((uint16_t*)a.out + t * a.ldo + c0, z);
+    }
+}
+
+// Eight columns of one row of the gated projections: g their gate, u their up part.
+template <class T>
+__device__ inline void finish_gated8(const LinearArgs& a, float (&g)[8], float (&u)[8], long t, int c0, float qs) {
+    if constexpr (T::bytes == 1) {
+        if (a.p_scale) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const f32x4 sg = *(const f32x4_u*)(a.p_scale + c0 + 4 * h);
+                const f32x4 su = *(const f32x4_u*)(a.p_scale + a.p_cols + c0 + 4 * h);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    g[4 * h + e] *= qs * sg[e];
+                    u[4 * h + e] *= qs * su[e];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                g[e] *= qs;
+                u[e] *= qs;
+            }
+        }
+    } else if (a.pre) {
+        uint16_t* p = (uint16_t*)a.pre + t * a.ldpre + c0;
+        store16<T>(p, g);
+        store16<T>(p + a.p_cols, u);
+    }
+    activate(g, a.act);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) g[e] *= u[e];
+    store16<T>((uint16_t*)a.out + t * a.ldo + c0, g);
+}
+
+// Epilogue of a wave's block of 64 P rows and 16 output rows (first output row t0):
+// c[i] are its four accumulator tiles, col0 the first output column of the block.
+template <class T, int LAYOUT, int EPI>
+__device__ inline void finish_block(const LinearArgs& a, f32x4 (&c)[4], int t0, int col0, int lane, int split) {
+    if constexpr (LAYOUT != ROWS_ROWS) transpose_groups(c);
+    const int g = lane >> 4;
+    const long t = t0 + (lane & 15);
+    if (t >= a.q_rows) return;
+    const float qs = T::bytes == 1 && a.q_scale ? a.q_scale[t] : 1.0f;
+    if constexpr (EPI == EPI_GATED) {
+        const int c0 = col0 + g * 8;
+        if (c0 >= a.p_cols) return;
+        float ga[8], up[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            ga[e] = c[e >> 2][e & 3];
+            up[e] = c[2 + (e >> 2)][e & 3];
+        }
+        finish_gated8<T>(a, ga, up, t, c0, qs);
+    } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int c0 = col0 + g * 16 + h * 8;
+            if (c0 >= a.p_cols) return;
+            if (a.partial) {
+                float* o = a.partial + ((long)split * a.q_rows + t) * a.p_cols + c0;
+                *(f32x4*)o = c[2 * h];
+                *(f32x4*)(o + 4) = c[2 * h + 1];
+            } else {
+                float z[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) z[e] = c[2 * h + (e >> 2)][e & 3];
+                finish8<T>(a, z, t, c0, qs);
+            }
+        }
+    }
+}
+
+// Tile order: workgroup b runs on XCD b % 8, so each XCD gets a contiguous band of tiles,
+// swept GROUP row blocks at a time for every column block, which keeps the operands that
+// one XCD's resident tiles share in its 4 MB L2.
+__device__ inline void tile_coords(int b, int n_p, int n_q, int& tp, int& tq) {
+    constexpr int GROUP = 8;
+    const int ntiles = n_p * n_q, xcd = b & 7, q8 = ntiles >> 3, r8 = ntiles & 7;
+    const int tile = xcd * q8 + (xcd < r8 ? xcd : r8) + (b >> 3);
+    const int grp = tile / (GROUP * n_p), gi = tile - grp * GROUP * n_p, gh = min(GROUP, n_q - grp * GROUP);
+    tp = gi / gh;
+    tq = grp * GROUP + gi % gh;
+}
+
+}  // namespace lin

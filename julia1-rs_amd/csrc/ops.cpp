@@ -161,4 +161,104 @@ int jh_op_attention_unsplit(const void* q, size_t ldq, const void* k, const void
     return op_attention(q, ldq, k, v, ldkv, out, ldo, tiles, ntiles, heads, window, scale, wide ? 8 : 4, false, stream);
 }
 
+// ---------------------------------------------------------------- RMS norm, linear layers, gated projections
+
+int jh_op_rms_norm(int x_type, const void* x, size_t ldx, int resid_type, const void* resid, size_t ldr,
+                   void* resid_out, size_t ldro, size_t rows, size_t hidden, const float* w, float eps, int out_type,
+                   void* out, size_t ldo, float* scales, float* rstd, void* stream) {
+    return jh_guarded([&] {
+        RmsNormArgs a{x_type, resid ? resid_type : x_type, out_type, x, (long)ldx, resid, (long)ldr, resid_out, (long)ldro,
+                      as_int(rows, "rows"), as_int(hidden, "hidden"), w, eps, out, (long)ldo, scales, rstd};
+        rms_norm(a, (hipStream_t)stream);
+    });
+}
+
+int jh_op_rms_norm_backward(int dy_type, const void* dy, size_t lddy, int s_type, const void* s, size_t lds,
+                            size_t rows, size_t hidden, const float* w, const float* rstd, int ds_type,
+                            const void* dres, size_t lddr, void* ds, size_t ldds, float* dw, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+    return jh_guarded([&] {
+        RmsNormGradArgs a{dy_type, s_type, ds_type, dy, (long)lddy, s, (long)lds, as_int(rows, "rows"),
+                          as_int(hidden, "hidden"), w, rstd, dres, (long)lddr, ds, (long)ldds, dw, (float*)workspace, 0};
+        rms_norm_backward(a, workspace_bytes, (hipStream_t)stream);
+    });
+}
+
+size_t jh_op_rms_norm_backward_workspace(size_t rows, size_t hidden) {
+    size_t bytes = 0;
+    jh_guarded([&] { bytes = rms_norm_backward_workspace(as_int(rows, "rows"), as_int(hidden, "hidden")); });
+    return bytes;
+}
+
+int jh_op_quantize_rows(int x_type, const void* x, size_t ldx, size_t rows, size_t cols, void* q, size_t ldq,
+                        float* scales, void* stream) {
+    return jh_guarded([&] {
+        RmsNormArgs a{x_type, x_type, JH_E4M3, x, (long)ldx, nullptr, 0, nullptr, 0, as_int(rows, "rows"),
+                      as_int(cols, "cols"), nullptr, 0.0f, q, (long)ldq, scales, nullptr};
+        quantize_rows(a, (hipStream_t)stream);
+    });
+}
+
+int jh_op_linear(int type, const void* x, size_t ldx, const float* x_scale, size_t rows, const void* w,
+                 const float* w_scale, size_t n, size_t k, const float* bias, int act, const void* resid, size_t ldr,
+                 int out_type, void* out, size_t ldo, void* pre, size_t ldp, void* stream) {
+    return jh_guarded([&] {
+        LinearArgs a{type, 0, 0, w, (long)k, x, (long)ldx, as_int(n, "n"), as_int(rows, "rows"), as_int(k, "k"), w_scale,
+                     x_scale, bias, act, resid, (long)ldr, out, (long)ldo, out_type == JH_F32, pre, (long)ldp};
+        linear_forward(a, rows, n, k, out_type, (hipStream_t)stream);
+    });
+}
+
+int jh_op_linear_backward(int type, const void* dy, size_t lddy, const void* x, size_t ldx, size_t rows, const void* w,
+                          size_t n, size_t k, int act, const void* pre, size_t ldp, void* dx, size_t lddx,
+                          int grad_type, void* dw, float* dbias, void* workspace, size_t workspace_bytes,
+                          void* stream) {
+    return jh_guarded([&] {
+        if (grad_type != type && grad_type != JH_F32)
+            throw jh_error(JH_ERR_INVALID, "linear_backward: dw has the operands' type or f32");
+        LinearGradArgs a{type, 0, act, dy, (long)lddy, pre, (long)ldp, x, (long)ldx, w, dx, (long)lddx,
+                         grad_type == JH_F32, dw, dbias, workspace, workspace_bytes};
+        linear_backward(a, rows, n, k, (hipStream_t)stream);
+    });
+}
+
+size_t jh_op_linear_backward_workspace(size_t rows, size_t n, size_t k, int act) {
+    size_t bytes = 0;
+    jh_guarded([&] { bytes = linear_backward_workspace(rows, n, k, act, false); });
+    return bytes;
+}
+
+int jh_op_gated_ffn(int type, const void* x, size_t ldx, const float* x_scale, size_t rows, const void* wi,
+                    const float* wi_scale, size_t inter, size_t k, int act, void* out, size_t ldo, void* gu,
+                    size_t ldgu, void* stream) {
+    return jh_guarded([&] {
+        LinearArgs a{type, 0, 1, wi, (long)k, x, (long)ldx, as_int(inter, "inter"), as_int(rows, "rows"), as_int(k, "k"),
+                     wi_scale, x_scale, nullptr, act, nullptr, 0, out, (long)ldo, 0, gu, (long)ldgu};
+        linear_forward(a, rows, inter, k, type == JH_E4M3 ? JH_BF16 : type, (hipStream_t)stream);
+    });
+}
+
+int jh_op_gated_ffn_backward(int type, const void* dh, size_t lddh, const void* gu, size_t ldgu, const void* x,
+                             size_t ldx, size_t rows, const void* wi, size_t inter, size_t k, int act, void* dx,
+                             size_t lddx, int grad_type, void* dwi, void* workspace, size_t workspace_bytes,
+                             void* stream) {
+    return jh_guarded([&] {
+        if (grad_type != type && grad_type != JH_F32)
+            throw jh_error(JH_ERR_INVALID, "gated_ffn_backward: dwi has the operands' type or f32");
+        if (inter > ((size_t)1 << 21)) throw jh_error(JH_ERR_INVALID, "gated_ffn_backward: too large");
+        LinearGradArgs a{type, 1, act, dh, (long)lddh, gu, (long)ldgu, x, (long)ldx, wi, dx, (long)lddx,
+                         grad_type == JH_F32, dwi, nullptr, workspace, workspace_bytes};
+        linear_backward(a, rows, 2 * inter, k, (hipStream_t)stream);
+    });
+}
+
+size_t jh_op_gated_ffn_backward_workspace(size_t rows, size_t inter, size_t k) {
+    size_t bytes = 0;
+    jh_guarded([&] {
+        if (inter > ((size_t)1 << 21)) throw jh_error(JH_ERR_INVALID, "gated_ffn_backward: too large");
+        bytes = linear_backward_workspace(rows, 2 * inter, k, JH_ACT_NONE, true);
+    });
+    return bytes;
+}
+
 }  // extern "C"

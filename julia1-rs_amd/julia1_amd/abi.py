@@ -32,6 +32,10 @@ EPI_BIAS_BF16 = 4
 EPI_BIAS_RELU_BF16 = 5
 EPI_BIAS_F32 = 6
 
+# element types and activations of jh_op_rms_norm, jh_op_linear and jh_op_gated_ffn
+F32, BF16, F16, E4M3 = range(4)
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = range(5)
+
 _f32p = C.POINTER(C.c_float)
 
 

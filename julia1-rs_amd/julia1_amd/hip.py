@@ -24,6 +24,9 @@ EXPORTS = (
     "jh_op_interleave_geglu",
     "jh_op_embed_ln", "jh_op_layer_norm", "jh_op_final_norm",
     "jh_op_gather_f32", "jh_op_scorer", "jh_op_attention", "jh_op_attention_wide", "jh_op_attention_unsplit",
+    "jh_op_rms_norm", "jh_op_rms_norm_backward", "jh_op_rms_norm_backward_workspace", "jh_op_quantize_rows",
+    "jh_op_linear", "jh_op_linear_backward", "jh_op_linear_backward_workspace",
+    "jh_op_gated_ffn", "jh_op_gated_ffn_backward", "jh_op_gated_ffn_backward_workspace",
 )
 
 
@@ -90,6 +93,22 @@ def lib():
         L.jh_op_attention.argtypes = [vp, sz, vp, vp, sz, vp, sz, vp, sz, sz, C.c_int, C.c_float, vp]
         L.jh_op_attention_wide.argtypes = L.jh_op_attention.argtypes
         L.jh_op_attention_unsplit.argtypes = L.jh_op_attention.argtypes[:-1] + [C.c_int, vp]
+        i32, f32 = C.c_int, C.c_float
+        L.jh_op_rms_norm.argtypes = [i32, vp, sz, i32, vp, sz, vp, sz, sz, sz, vp, f32, i32, vp, sz, vp, vp, vp]
+        L.jh_op_rms_norm_backward.argtypes = [i32, vp, sz, i32, vp, sz, sz, sz, vp, vp, i32, vp, sz, vp, sz, vp, vp, sz,
+                                              vp]
+        L.jh_op_quantize_rows.argtypes = [i32, vp, sz, sz, sz, vp, sz, vp, vp]
+        L.jh_op_linear.argtypes = [i32, vp, sz, vp, sz, vp, vp, sz, sz, vp, i32, vp, sz, i32, vp, sz, vp, sz, vp]
+        L.jh_op_linear_backward.argtypes = [i32, vp, sz, vp, sz, sz, vp, sz, sz, i32, vp, sz, vp, sz, i32, vp, vp, vp,
+                                            sz, vp]
+        L.jh_op_gated_ffn.argtypes = [i32, vp, sz, vp, sz, vp, vp, sz, sz, i32, vp, sz, vp, sz, vp]
+        L.jh_op_gated_ffn_backward.argtypes = [i32, vp, sz, vp, sz, vp, sz, sz, vp, sz, sz, i32, vp, sz, i32, vp, vp,
+                                               sz, vp]
+        L.jh_op_rms_norm_backward_workspace.argtypes = [sz, sz]
+        L.jh_op_linear_backward_workspace.argtypes = [sz, sz, sz, i32]
+        L.jh_op_gated_ffn_backward_workspace.argtypes = [sz, sz, sz]
+        for name in ("rms_norm", "linear", "gated_ffn"):
+            getattr(L, f"jh_op_{name}_backward_workspace").restype = sz
         _lib = L
     return _lib
 
@@ -325,3 +344,178 @@ def op_attention(q, ldq, k, v, ldkv, out, ldo, tiles, heads, window, scale=0.125
     fn = lib().jh_op_attention_wide if wide else lib().jh_op_attention
     check(fn(_dp(q), ldq, _dp(k), _dp(v), ldkv, _dp(out), ldo, _dp(tiles), tiles.shape[0], heads, window, scale,
              stream))
+
+
+# ---------------------------------------------------------------- RMS norm, linear layers, gated projections
+
+ACTS = {"none": abi.ACT_NONE, "relu": abi.ACT_RELU, "gelu": abi.ACT_GELU, "gelu_tanh": abi.ACT_GELU_TANH,
+        "silu": abi.ACT_SILU}
+_TYPES = None
+
+
+def _type(t):
+    """The element type code of a torch tensor."""
+    global _TYPES
+    if _TYPES is None:
+        import torch
+        _TYPES = {torch.float32: abi.F32, torch.bfloat16: abi.BF16, torch.float16: abi.F16,
+                  torch.float8_e4m3fn: abi.E4M3}
+    code = _TYPES.get(t.dtype)
+    if code is None:
+        raise HipError(abi.JH_ERR_INVALID, f"no such element type: {t.dtype}")
+    return code
+
+
+def _invalid(msg):
+    raise HipError(abi.JH_ERR_INVALID, msg)
+
+
+def _mat(name, t, rows, cols, dev, dtype=None):
+    """(address, row stride) of a 2-D tensor of the wanted shape, device and type; (None, 0) for None."""
+    if t is None:
+        return None, 0
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
+        _invalid(f"{name}: shape {tuple(t.shape)}, expected {(rows, cols)}")
+    ld = t.stride(0)
+    if (cols > 1 and t.stride(1) != 1) or ld < 0 or t.device != dev:
+        _invalid(f"{name}: needs contiguous rows on {dev}")
+    if dtype is not None and t.dtype != dtype:
+        _invalid(f"{name}: {t.dtype}, expected {dtype}")
+    return t.data_ptr(), max(ld, cols) if rows <= 1 else ld
+
+
+def _vec(name, t, n, dev):
+    """Address of a contiguous f32 vector of n values; None for None."""
+    if t is None:
+        return None
+    import torch
+    if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous() or t.device != dev:
+        _invalid(f"{name}: needs {n} contiguous float32 values on {dev}")
+    return t.data_ptr()
+
+
+def _weight(name, t, rows, cols, dev, dtype):
+    if t is not None and not t.is_contiguous():
+        _invalid(f"{name}: needs a contiguous matrix")
+    return _mat(name, t, rows, cols, dev, dtype)[0]
+
+
+def _space(t, dev):
+    if t is None:
+        return None, 0
+    if not t.is_contiguous() or t.device != dev:
+        _invalid(f"workspace: needs contiguous memory on {dev}")
+    return t.data_ptr(), t.numel() * t.element_size()
+
+
+def _act(name):
+    if name not in ACTS:
+        _invalid(f"unknown activation {name!r}")
+    return ACTS[name]
+
+
+def op_rms_norm(x, w, eps, out, resid=None, resid_out=None, scales=None, rstd=None, stream=None):
+    """jh_op_rms_norm: out = RMS norm of s = x + resid, times w; s goes to resid_out (which may be resid).  out of
+    torch.float8_e4m3fn takes e4m3 codes and scales their f32 scale per row; rstd (f32) is kept for the backward."""
+    (rows, h), dev = x.shape, x.device
+    (xp, ldx), (op, ldo) = _mat("x", x, rows, h, dev), _mat("out", out, rows, h, dev)
+    rp, ldr = _mat("resid", resid, rows, h, dev)
+    sp, lds = _mat("resid_out", resid_out, rows, h, dev, None if resid is None else resid.dtype)
+    check(lib().jh_op_rms_norm(_type(x), xp, ldx, 0 if resid is None else _type(resid), rp, ldr, sp, lds, rows, h,
+                               _vec("w", w, h, dev), eps, _type(out), op, ldo, _vec("scales", scales, rows, dev),
+                               _vec("rstd", rstd, rows, dev), stream))
+
+
+def op_rms_norm_backward(dy, s, w, rstd, ds, dw=None, workspace=None, dres=None, stream=None):
+    """jh_op_rms_norm_backward: ds (+ dres) and dw from dy, with s = resid_out (or x) and rstd of op_rms_norm; dw
+    needs a workspace tensor of rms_norm_backward_workspace(rows, hidden) bytes."""
+    (rows, h), dev = dy.shape, dy.device
+    (yp, ldy), (sp, lds) = _mat("dy", dy, rows, h, dev), _mat("s", s, rows, h, dev)
+    dp, ldd = _mat("ds", ds, rows, h, dev)
+    rp, ldr = _mat("dres", dres, rows, h, dev, ds.dtype)
+    wp, wb = _space(workspace, dev)
+    check(lib().jh_op_rms_norm_backward(_type(dy), yp, ldy, _type(s), sp, lds, rows, h, _vec("w", w, h, dev),
+                                        _vec("rstd", rstd, rows, dev), _type(ds), rp, ldr, dp, ldd,
+                                        _vec("dw", dw, h, dev), wp, wb, stream))
+
+
+def rms_norm_backward_workspace(rows, hidden) -> int:
+    return _bytes(lib().jh_op_rms_norm_backward_workspace(rows, hidden))
+
+
+def _bytes(n):
+    if lib().jh_last_error():
+        raise HipError(abi.JH_ERR_INVALID, lib().jh_last_error().decode())
+    return n
+
+
+def op_quantize_rows(x, q, scales, stream=None):
+    """jh_op_quantize_rows: e4m3 codes q (torch.float8_e4m3fn) of x's rows and their f32 scales."""
+    import torch
+    (rows, n), dev = x.shape, x.device
+    (xp, ldx), (qp, ldq) = _mat("x", x, rows, n, dev), _mat("q", q, rows, n, dev, torch.float8_e4m3fn)
+    check(lib().jh_op_quantize_rows(_type(x), xp, ldx, rows, n, qp, ldq, _vec("scales", scales, rows, dev), stream))
+
+
+def op_linear(x, w, out, bias=None, act="none", resid=None, x_scale=None, w_scale=None, pre=None, stream=None):
+    """jh_op_linear: out = act(x w^T + bias) + resid; x and w of one type (bf16, f16, or float8_e4m3fn with x_scale and
+    w_scale), out f32 or their type (bf16 for e4m3); resid may be out; pre keeps x w^T + bias for the backward."""
+    (rows, k), dev = x.shape, x.device
+    n = w.shape[0]
+    (xp, ldx), (op, ldo) = _mat("x", x, rows, k, dev), _mat("out", out, rows, n, dev)
+    (rp, ldr), (pp, ldp) = _mat("resid", resid, rows, n, dev, out.dtype), _mat("pre", pre, rows, n, dev, x.dtype)
+    check(lib().jh_op_linear(_type(x), xp, ldx, _vec("x_scale", x_scale, rows, dev), rows,
+                             _weight("w", w, n, k, dev, x.dtype), _vec("w_scale", w_scale, n, dev), n, k,
+                             _vec("bias", bias, n, dev), _act(act), rp, ldr, _type(out), op, ldo, pp, ldp, stream))
+
+
+def op_linear_backward(dy, x, w, workspace, act="none", pre=None, dx=None, dw=None, dbias=None, stream=None):
+    """jh_op_linear_backward: whichever of dx, dw (f32 or x's type) and dbias (f32) are given, from dy and (act not
+    "none") pre; workspace of linear_backward_workspace(rows, n, k, act) bytes."""
+    (rows, n), dev = dy.shape, dy.device
+    k = w.shape[1]
+    (yp, ldy), (xp, ldx) = _mat("dy", dy, rows, n, dev), _mat("x", x, rows, k, dev, dy.dtype)
+    (pp, ldp), (dp, ldd) = _mat("pre", pre, rows, n, dev, dy.dtype), _mat("dx", dx, rows, k, dev, dy.dtype)
+    wp, wb = _space(workspace, dev)
+    check(lib().jh_op_linear_backward(_type(dy), yp, ldy, xp, ldx, rows, _weight("w", w, n, k, dev, dy.dtype), n, k,
+                                      _act(act), pp, ldp, dp, ldd, _type(dy if dw is None else dw),
+                                      _weight("dw", dw, n, k, dev, None), _vec("dbias", dbias, n, dev), wp, wb, stream))
+
+
+def linear_backward_workspace(rows, n, k, act="none") -> int:
+    return _bytes(lib().jh_op_linear_backward_workspace(rows, n, k, _act(act)))
+
+
+def op_gated_ffn(x, wi, out, act="gelu", x_scale=None, w_scale=None, gu=None, stream=None):
+    """jh_op_gated_ffn: out = act(x Wg^T) * (x Wu^T), wi = [Wg; Wu]; types as op_linear (out of x's type, bf16 for
+    e4m3); gu [rows, 2 inter] keeps both projections for the backward."""
+    (rows, k), dev = x.shape, x.device
+    n = wi.shape[0]
+    if n % 2:
+        _invalid("wi: needs an even number of rows")
+    half = None if _type(x) == abi.E4M3 else x.dtype
+    (xp, ldx), (op, ldo) = _mat("x", x, rows, k, dev), _mat("out", out, rows, n // 2, dev, half)
+    if half is None and _type(out) != abi.BF16:
+        _invalid("out: e4m3 operands give bfloat16")
+    gp, ldg = _mat("gu", gu, rows, n, dev, x.dtype)
+    check(lib().jh_op_gated_ffn(_type(x), xp, ldx, _vec("x_scale", x_scale, rows, dev), rows,
+                                _weight("wi", wi, n, k, dev, x.dtype), _vec("w_scale", w_scale, n, dev), n // 2, k,
+                                _act(act), op, ldo, gp, ldg, stream))
+
+
+def op_gated_ffn_backward(dh, gu, x, wi, workspace, act="gelu", dx=None, dw=None, stream=None):
+    """jh_op_gated_ffn_backward: dx and / or dw (of wi; f32 or x's type) from dh and gu; workspace of
+    gated_ffn_backward_workspace(rows, inter, k) bytes."""
+    (rows, inter), dev = dh.shape, dh.device
+    k = wi.shape[1]
+    (hp, ldh), (gp, ldg) = _mat("dh", dh, rows, inter, dev), _mat("gu", gu, rows, 2 * inter, dev, dh.dtype)
+    (xp, ldx), (dp, ldd) = _mat("x", x, rows, k, dev, dh.dtype), _mat("dx", dx, rows, k, dev, dh.dtype)
+    wp, wb = _space(workspace, dev)
+    check(lib().jh_op_gated_ffn_backward(_type(dh), hp, ldh, gp, ldg, xp, ldx, rows,
+                                         _weight("wi", wi, 2 * inter, k, dev, dh.dtype), inter, k, _act(act), dp, ldd,
+                                         _type(dh if dw is None else dw), _weight("dw", dw, 2 * inter, k, dev, None),
+                                         wp, wb, stream))
+
+
+def gated_ffn_backward_workspace(rows, inter, k) -> int:
+    return _bytes(lib().jh_op_gated_ffn_backward_workspace(rows, inter, k))
