@@ -244,9 +244,11 @@ void linear_forward(const LinearArgs& a, size_t rows, size_t n, size_t k, int ou
 void linear_backward(const LinearGradArgs& a, size_t rows, size_t n, size_t k, hipStream_t stream);
 size_t linear_backward_workspace(size_t rows, size_t n, size_t k, int act, bool gated);
 
-// One kernel each: 128 x 128 tiles, and few rows.
-void launch_linear_tile(const LinearArgs& a, hipStream_t stream);
-void launch_linear_small(const LinearArgs& a, hipStream_t stream);
+// One kernel each: 256 x 256 tiles, smaller tiles, and few rows.
+void launch_linear_wide(const LinearArgs& a, hipStream_t stream);  // not e4m3 operands with an FP32 output
+enum class LinearTile { Small, Group, Deep, Pair };  // see linear_tile.hip
+void launch_linear_tile(const LinearArgs& a, LinearTile tile, hipStream_t stream);
+void launch_linear_small(const LinearArgs& a, hipStream_t stream);  // at most 16 rows, k contiguous
 
 void rms_norm(const RmsNormArgs& a, hipStream_t stream);
 void quantize_rows(const RmsNormArgs& a, hipStream_t stream);

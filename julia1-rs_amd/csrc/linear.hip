@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "linear.hpp"
 
@@ -138,30 +139,97 @@ unsigned blocks_of(long items, const char* what) {
 
 long round_up(long v, long to) { return (v + to - 1) / to * to; }
 
-// ---------------------------------------------------------------- splits of the contraction
+// ---------------------------------------------------------------- choice of kernel
 
-long tiles_of(const LinearArgs& a) {
-    const long pw = a.gated ? 64 : 128;
-    return ((a.p_cols + pw - 1) / pw) * ((a.q_rows + 127L) / 128);
+long steps_of(const LinearArgs& a) {
+    const long es = a.type == JH_E4M3 ? 1 : 2;
+    return (a.k * es + STEP_BYTES - 1L) / STEP_BYTES;
 }
-long steps_of(const LinearArgs& a) { return (a.k + STEP_ROWS - 1L) / STEP_ROWS; }
+long tiles_of(const LinearArgs& a, int p, int q) {
+    const long cols = a.gated ? 2L * a.p_cols : a.p_cols;
+    return ((cols + p - 1) / p) * ((a.q_rows + q - 1L) / q);
+}
 
-// Into how many parts a gradient product's contraction is cut: as many as the 512 resident
-// workgroups have room for, of eight K steps at least, with the FP32 parts under 16 outputs
-// and 48 MiB.
-constexpr int MAX_SPLITS = 16;
-constexpr long SPLIT_BYTES = 48L << 20;
-int splits_of(const LinearArgs& a) {
-    const long out = (long)a.q_rows * a.p_cols * 4;
-    long s = std::min<long>(MAX_SPLITS, 512 / std::max(1L, tiles_of(a)));
-    s = std::min(s, steps_of(a) / 8);
-    s = std::min(s, SPLIT_BYTES / std::max(1L, out));
-    return (int)std::max(1L, s);
+// What a launch of each kernel takes, in us, from its number of tiles and of K steps: a start
+// and an end per round of tiles (launch, first loads, epilogue) and a time per step that grows
+// with the CUs at work (shared L2 and power).  The constants are fits to times of bf16 products
+// on an MI355X (256 CUs; us, the kernel taken in brackets):
+//
+//   rows x n x k         Small   Group   Deep    Pair    256 x 256
+//   512 x 768 x 768      [6.2]   7.5     9.1     11.3    20.6
+//   128 x 1024 x 4096    16.8    [14.5]  28.3    36.6    69.1
+//   1024 x 1024 x 4096   [19.1]  21.1    29.2    46.4    69.8
+//   1024 x 4096 x 1024   17.5    26.3    [13.4]  15.6    25.4
+//   2048 x 4096 x 4096   105     147     73.0    [60.3]  71.8
+//   4096 x 4096 x 4096   203     291     140     117     [96.3]
+//   9482 x 4096 x 1024   149     246     108     88.7    [81.9]
+enum { SMALL, GROUP, DEEP, PAIR, WIDE, KERNELS };
+constexpr double CUS = 256;
+
+double cost(int kernel, const LinearArgs& a, long splits) {
+    const double s = (double)((steps_of(a) + splits - 1) / splits);
+    auto rounds = [](double t, double slots) { return std::ceil(t / slots); };
+    auto load = [](double t) { return std::min(1.0, t / CUS); };
+    switch (kernel) {
+        case SMALL: {
+            const double t = (double)(tiles_of(a, 64, 64) * splits);
+            return t <= CUS ? 3.0 + 0.22 * s : rounds(t, 2 * CUS) * (0.42 * s + 2.0) + 1.0;
+        }
+        case GROUP: {
+            const double t = (double)(tiles_of(a, 64, 64) * splits);
+            return rounds(t, CUS) * (std::ceil(s / 4) * (t <= 64 ? 0.58 : 0.98) + 3.5) + 1.5;
+        }
+        case DEEP: {
+            const double t = (double)(tiles_of(a, 128, 128) * splits);
+            return rounds(t, CUS) * (s * (0.35 + 0.19 * load(t)) + 3.0) + 1.0;
+        }
+        case PAIR: {
+            const double t = (double)(tiles_of(a, 128, 128) * splits);
+            return rounds(t, 2 * CUS) * (s * (t <= CUS ? 0.65 : 0.88) + 3.5) + 1.0;
+        }
+        default: {
+            const double t = (double)(tiles_of(a, 256, 256) * splits);
+            return rounds(t, CUS) * (s * (1.0 + 0.35 * load(t)) + 6.0) + 1.0;
+        }
+    }
+}
+
+struct Choice {
+    int kernel;
+    int splits;
+};
+
+// The cheapest kernel and, for gradients, number of parts of the contraction, whose FP32 sums
+// take `splits` outputs' worth of memory (at most 16, and 48 MiB) and one more kernel.
+constexpr long MAX_SPLITS = 16, SPLIT_BYTES = 48L << 20, MIN_STEPS = 4;
+Choice pick(const LinearArgs& a, bool gradient) {
+    Choice best{PAIR, 1};
+    double least = 1e30;
+    const double out = (double)a.q_rows * a.p_cols * 4;
+    for (long splits = 1; splits <= (gradient ? MAX_SPLITS : 1); splits += splits < 4 ? 1 : splits < 8 ? 2 : 4) {
+        if (splits > 1 && (steps_of(a) < splits * MIN_STEPS || out * splits > SPLIT_BYTES)) break;
+        const double sum = splits > 1 ? 2.5 + (splits + 1) * out / 4.5e6 : 0.0;
+        for (int kernel = 0; kernel < KERNELS; ++kernel) {
+            if (kernel == WIDE && a.type == JH_E4M3 && a.out_f32) continue;  // has no bf16 fragments of e4m3
+            const double c = cost(kernel, a, splits) + sum;
+            if (c < least) {
+                least = c;
+                best = {kernel, (int)splits};
+            }
+        }
+    }
+    return best;
 }
 
 long partial_bytes(const LinearArgs& a) {
-    const int s = splits_of(a);
+    const int s = pick(a, true).splits;
     return s > 1 ? round_up((long)s * a.q_rows * a.p_cols * 4, 256) : 0;
+}
+
+void launch(int kernel, const LinearArgs& a, hipStream_t s) {
+    if (kernel == WIDE) launch_linear_wide(a, s);
+    else launch_linear_tile(a, kernel == SMALL ? LinearTile::Small : kernel == GROUP ? LinearTile::Group
+                               : kernel == DEEP ? LinearTile::Deep : LinearTile::Pair, s);
 }
 
 template <class T>
@@ -172,23 +240,26 @@ void split_sum(const LinearArgs& a, hipStream_t s) {
     HIP_CHECK(hipGetLastError());
 }
 
+// Up to 16 rows, W streams past them from memory (16 x 4096 x 4096: 10.1 us, 16.5 on 64 x 64
+// tiles; 17 to 32 rows, two blocks of them, took 18.2 against 17.6).
+constexpr int STREAM_ROWS = 16;
+
 void run(LinearArgs a, hipStream_t s) {
-    if (a.q_rows == 0) return;
     a.splits = 1;
     a.split_steps = 0x7fffffff;
-    if (a.layout == ROWS_ROWS && a.q_rows <= 64) launch_linear_small(a, s);
-    else launch_linear_tile(a, s);
+    if (a.q_rows <= STREAM_ROWS) launch_linear_small(a, s);
+    else launch(pick(a, false).kernel, a, s);
 }
 
 // A gradient product, its contraction split where that fills the GPU.
 void run_gradient(LinearArgs a, float* partial, hipStream_t s) {
     if (a.q_rows == 0) return;
-    const int splits = splits_of(a);
-    a.split_steps = (int)((steps_of(a) + splits - 1) / splits);
-    a.splits = splits;
-    a.partial = splits > 1 ? partial : nullptr;
-    launch_linear_tile(a, s);
-    if (splits == 1) return;
+    const Choice c = pick(a, true);
+    a.split_steps = (int)((steps_of(a) + c.splits - 1) / c.splits);
+    a.splits = c.splits;
+    a.partial = c.splits > 1 ? partial : nullptr;
+    launch(c.kernel, a, s);
+    if (c.splits == 1) return;
     if (a.type == JH_BF16) split_sum<Bf16>(a, s);
     else split_sum<F16>(a, s);
 }
@@ -206,13 +277,16 @@ int type_bytes(int type) { return type == JH_F32 ? 4 : type == JH_E4M3 ? 1 : 2; 
 // ---------------------------------------------------------------- shared argument checks
 
 void check_matrix(const char* op, const char* name, const void* p, size_t ld, size_t rows, size_t cols, int type) {
-    const size_t unit = 16 / type_bytes(type);
-    const std::string n = std::string(op) + ": " + name;
-    if (!p) throw jh_error(JH_ERR_INVALID, n + " is null");
-    if ((uintptr_t)p & 15) throw jh_error(JH_ERR_INVALID, n + " is not 16-byte aligned");
-    if (ld < cols && rows > 1) throw jh_error(JH_ERR_INVALID, n + ": row stride below its columns");
-    if (rows > 1 && ld % unit) throw jh_error(JH_ERR_INVALID, n + ": rows are not 16-byte aligned");
-    if (ld > ((size_t)1 << 22) / type_bytes(type)) throw jh_error(JH_ERR_INVALID, n + ": row stride over 4 MiB");
+    const size_t bytes = type_bytes(type);
+    const char* what = !p                                          ? " is null"
+                       : (uintptr_t)p & 15                         ? " is not 16-byte aligned"
+                       : rows <= 1                                 ? nullptr
+                       : ld < cols                                 ? ": row stride below its columns"
+                       : ld > ((size_t)1 << 22) / bytes            ? ": row stride over 4 MiB"
+                       : ld * bytes % 16                           ? ": rows are not 16-byte aligned"
+                                                                   : nullptr;
+    if (!what && cols * bytes > ((size_t)1 << 22)) what = ": rows over 4 MiB";
+    if (what) throw jh_error(JH_ERR_INVALID, std::string(op) + ": " + name + what);
 }
 
 Span span_of(const void* p, size_t ld, size_t rows, size_t cols, int type) {

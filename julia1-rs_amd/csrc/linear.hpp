@@ -21,6 +21,7 @@ typedef int32_t i32x8 __attribute__((ext_vector_type(8)));
 typedef f32x4 f32x4_u __attribute__((aligned(4)));  // bias and scales need no more than their type's alignment
 typedef short lin_s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) lin_s16x4 lds_lin_s16x4;
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 
 namespace lin {
 
@@ -79,7 +80,7 @@ struct E4m3 : Bf16 {
         return i32x8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
     }
     __device__ static f32x4 mfma(const Frag& a, const Frag& b, f32x4 c) {
-        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
     }
 };
 
@@ -140,7 +141,13 @@ __device__ inline void activate(float (&v)[N], int act) {
 // ---------------------------------------------------------------- operand staging
 
 __device__ constexpr int row_swz(int r) { return (r >> 1) & 7; }
-__device__ constexpr int col_swz(int k) { return ((k & 3) << 1) | (((k >> 3) & 1) << 3); }
+// 16-byte chunk swizzle of contraction row k where a staged row holds 128 columns (256 bytes,
+// all 64 banks) or 64: the transposing reads of half a wave touch rows k .. k+3 and k+8 .. k+11,
+// two chunks each, which land on distinct banks.
+template <int COLS>
+__device__ constexpr int col_swz(int k) {
+    return COLS >= 128 ? ((k & 3) << 1) | (((k >> 3) & 1) << 3) : (((k >> 1) & 1) << 1) | (((k >> 3) & 1) << 2);
+}
 
 // Which P row (output column, counted from the tile's first) LDS row `r` holds, so that a
 // lane's four accumulator tiles of a 64-row block are 16 consecutive columns: row
@@ -167,35 +174,62 @@ __device__ inline void dma16(uint32_t lds, uint32_t voff, i32x4 rsrc, uint32_t s
 
 // ---------------------------------------------------------------- fragments
 
-// k-contiguous operand staged as 128-byte rows, 16-byte chunks XOR-swizzled by the row:
-// the fragment of K half `h` (chunks 4h + g) of row `r`.
-__device__ inline u32x4 row_frag(const uint8_t* part, int r, int h, int g) {
-    return *(const u32x4*)(part + r * 128 + (((h * 4 + g) ^ row_swz(r)) << 4));
-}
+// Reads a wave's fragments of an operand from LDS.  A lane keeps a few addresses, to which
+// the place of the part in LDS (and of the tile in the part) adds a constant that goes into
+// the read's own offset; they are made opaque, or the compiler keeps an address for every
+// read.
+//
+// k contiguous: 128-byte rows, 16-byte chunks XOR-swizzled by the row; the fragment of row r
+// and K half h is chunk 4h + g.
+// k as row index: 64 rows of WIDTH columns, 16-byte chunks XOR-swizzled by the row.
+// The fragment of 16 columns and K half h is k = 32h + 8g + (0..7), by two transposing reads
+// (in each 16 lanes, lane j addresses row j / 4 and columns 4 (j % 4); lane i receives four
+// rows of column i).  TILES: the 16-column tiles that the wave reads of a part.
+template <class T, bool COLS, int TILES, int WIDTH = 128>
+struct FragReader {
+    static constexpr int N = COLS ? TILES : 1;
+    uint32_t at[N];
 
-// Operand with k as row index, staged as 64 rows of 128 columns (256 bytes): the fragment
-// of columns c0 .. c0+15 and K half `h`, k = 32h + 8g + (0..7), by two transposing reads
-// (in each 16 lanes, lane j addresses row j / 4, columns 4 (j % 4); lane i receives four
-// rows of column i).
-__device__ inline u32x4 col_frag(const uint8_t* part, int c0, int h, int lane) {
-    const int g = lane >> 4, k = h * 32 + g * 8 + ((lane & 15) >> 2), q = (c0 >> 3) + ((lane & 3) >> 1);
-    const uint8_t* p0 = part + k * 256 + ((q ^ col_swz(k)) << 4) + (lane & 1) * 8;
-    const uint8_t* p1 = p0 + 4 * 256;  // col_swz(k + 4) == col_swz(k): k % 8 < 4
-    const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_lin_s16x4*)p0));
-    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_lin_s16x4*)p1));
-    return u32x4{lo[0], lo[1], hi[0], hi[1]};
-}
-
-// The fragment of 16 operand rows (or columns) from `first` of a staged part.
-template <class T, bool COLS>
-__device__ inline typename T::Frag frag(const uint8_t* part, int first, int lane) {
-    if constexpr (COLS) {
-        return T::make(col_frag(part, first, 0, lane), col_frag(part, first, 1, lane));
-    } else {
-        const int r = first + (lane & 15), g = lane >> 4;
-        return T::make(row_frag(part, r, 0, g), row_frag(part, r, 1, g));
+    // `first`: the wave's first row (column) within a part; `lds`: the LDS address of the part
+    // that offset 0 stands for.
+    __device__ FragReader(const uint8_t* lds, int first, int lane) {
+        const uint32_t base = (uint32_t)(uintptr_t)lds;
+        const int g = lane >> 4, m = lane & 15;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            if constexpr (COLS) {
+                // the swizzle has period 4 in k but for bit 3: the same for k + 4 and k + 32
+                const int k = g * 8 + (m >> 2), q = ((first + n * 16) >> 3) + ((lane & 3) >> 1);
+                at[n] = base + k * (2 * WIDTH) + ((q ^ col_swz<WIDTH>(k)) << 4) + (lane & 1) * 8;
+            } else {
+                const int r = first + m;
+                at[n] = base + r * 128 + ((g ^ row_swz(r)) << 4);
+            }
+            asm volatile("" : "+v"(at[n]));
+        }
     }
-}
+
+    // The fragment as its two halves' bytes, for T::make.
+    struct Raw {
+        u32x4 lo, hi;
+        __device__ typename T::Frag frag() const { return T::make(lo, hi); }
+    };
+    __device__ Raw read(int offset, int tile) const {
+        if constexpr (COLS) {
+            u32x2 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                v[i] = __builtin_bit_cast(
+                    u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                               (lds_lin_s16x4*)(at[tile] + offset + ((i >> 1) * 32 + (i & 1) * 4) * (2 * WIDTH))));
+            return {u32x4{v[0][0], v[0][1], v[1][0], v[1][1]}, u32x4{v[2][0], v[2][1], v[3][0], v[3][1]}};
+        } else {
+            // the second half's chunk: 4 of 8 chunks on under the XOR swizzle
+            return {*(const lds_u32x4*)(at[0] + offset + tile * 2048),
+                    *(const lds_u32x4*)((at[0] ^ 64) + offset + tile * 2048)};
+        }
+    }
+};
 
 // ---------------------------------------------------------------- epilogue
 
@@ -236,53 +270,69 @@ __device__ inline void store16(void* dst, const float (&v)[N]) {
                                               T::pack(v[c + 4], v[c + 5]), T::pack(v[c + 6], v[c + 7])};
 }
 
-// Eight columns of one output row: c0 .. c0+7 (c0 % 8 == 0 and c0 < a.p_cols).
+// What the epilogue needs of eight output columns, whatever the row: loaded once per lane.
 template <class T>
-__device__ inline void finish8(const LinearArgs& a, float (&z)[8], long t, int c0, float qs) {
-    if constexpr (T::bytes == 1) {
-        if (a.p_scale) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const f32x4 s = *(const f32x4_u*)(a.p_scale + c0 + 4 * h);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) z[4 * h + e] *= qs * s[e];
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) z[e] *= qs;
-        }
-    }
-    if (a.bias) {
+struct ColumnTerms {
+    f32x4 bias[2], scale[2];
+
+    // Columns past the last read the last eight (nothing of them is stored).
+    __device__ void load(const LinearArgs& a, int c0, const float* p_scale) {
+        const int c = min(c0, a.p_cols - 8);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const f32x4 b = *(const f32x4_u*)(a.bias + c0 + 4 * h);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) z[4 * h + e] += b[e];
+            bias[h] = a.bias ? *(const f32x4_u*)(a.bias + c + 4 * h) : f32x4{0, 0, 0, 0};
+            if constexpr (T::bytes == 1) scale[h] = p_scale ? *(const f32x4_u*)(p_scale + c + 4 * h) : f32x4{1, 1, 1, 1};
         }
     }
+    __device__ void apply(const LinearArgs& a, float (&z)[8], float qs) const {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if constexpr (T::bytes == 1) z[e] *= qs * scale[e >> 2][e & 3];
+            if (a.bias) z[e] += bias[e >> 2][e & 3];
+        }
+    }
+};
+
+// The residual of eight columns of one row, raw.
+struct Resid8 {
+    u32x4 v[2];
+    __device__ void load(const LinearArgs& a, long t, int c0) {
+        const long at = min(t, (long)a.q_rows - 1) * a.ldr + min(c0, a.p_cols - 8);
+        if (a.out_f32) {
+            v[0] = *(const u32x4*)((const float*)a.resid + at);
+            v[1] = *(const u32x4*)((const float*)a.resid + at + 4);
+        } else {
+            v[0] = *(const u32x4*)((const uint16_t*)a.resid + at);
+        }
+    }
+};
+
+// Eight columns of one output row from their sums z: c0 .. c0+7.
+template <class T>
+__device__ inline void finish8(const LinearArgs& a, float (&z)[8], long t, int c0, float qs, const ColumnTerms<T>& col,
+                               const Resid8& resid) {
+    col.apply(a, z, qs);
     if constexpr (T::bytes == 2)
         if (a.pre) store16<T>((uint16_t*)a.pre + t * a.ldpre + c0, z);
     activate(z, a.act);
     if (a.out_f32) {
-        float* o = (float*)a.out + t * a.ldo + c0;
         if (a.resid) {
-            const float* r = (const float*)a.resid + t * a.ldr + c0;
-            const f32x4 r0 = *(const f32x4*)r, r1 = *(const f32x4*)(r + 4);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                z[e] += r0[e];
-                z[4 + e] += r1[e];
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t r = resid.v[e >> 2][e & 3];
+                z[e] += __builtin_bit_cast(float, r);
             }
         }
+        float* o = (float*)a.out + t * a.ldo + c0;
         *(f32x4*)o = f32x4{z[0], z[1], z[2], z[3]};
         *(f32x4*)(o + 4) = f32x4{z[4], z[5], z[6], z[7]};
     } else {
         if (a.resid) {
-            const u32x4 r = *(const u32x4*)((const uint16_t*)a.resid + t * a.ldr + c0);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                z[2 * e] += T::lo(r[e]);
-                z[2 * e + 1] += T::hi(r[e]);
+                const uint32_t r = resid.v[0][e];
+                z[2 * e] += T::lo(r);
+                z[2 * e + 1] += T::hi(r);
             }
         }
         store16<T>((uint16_t*)a.out + t * a.ldo + c0, z);
@@ -291,26 +341,11 @@ __device__ inline void finish8(const LinearArgs& a, float (&z)[8], long t, int c
 
 // Eight columns of one row of the gated projections: g their gate, u their up part.
 template <class T>
-__device__ inline void finish_gated8(const LinearArgs& a, float (&g)[8], float (&u)[8], long t, int c0, float qs) {
+__device__ inline void finish_gated8(const LinearArgs& a, float (&g)[8], float (&u)[8], long t, int c0, float qs,
+                                     const ColumnTerms<T>& gate, const ColumnTerms<T>& up) {
     if constexpr (T::bytes == 1) {
-        if (a.p_scale) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const f32x4 sg = *(const f32x4_u*)(a.p_scale + c0 + 4 * h);
-                const f32x4 su = *(const f32x4_u*)(a.p_scale + a.p_cols + c0 + 4 * h);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    g[4 * h + e] *= qs * sg[e];
-                    u[4 * h + e] *= qs * su[e];
-                }
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                g[e] *= qs;
-                u[e] *= qs;
-            }
-        }
+        gate.apply(a, g, qs);
+        up.apply(a, u, qs);
     } else if (a.pre) {
         uint16_t* p = (uint16_t*)a.pre + t * a.ldpre + c0;
         store16<T>(p, g);
@@ -322,41 +357,61 @@ __device__ inline void finish_gated8(const LinearArgs& a, float (&g)[8], float (
     store16<T>((uint16_t*)a.out + t * a.ldo + c0, g);
 }
 
-// Epilogue of a wave's block of 64 P rows and 16 output rows (first output row t0):
-// c[i] are its four accumulator tiles, col0 the first output column of the block.
-template <class T, int LAYOUT, int EPI>
-__device__ inline void finish_block(const LinearArgs& a, f32x4 (&c)[4], int t0, int col0, int lane, int split) {
-    if constexpr (LAYOUT != ROWS_ROWS) transpose_groups(c);
-    const int g = lane >> 4;
-    const long t = t0 + (lane & 15);
-    if (t >= a.q_rows) return;
-    const float qs = T::bytes == 1 && a.q_scale ? a.q_scale[t] : 1.0f;
-    if constexpr (EPI == EPI_GATED) {
-        const int c0 = col0 + g * 8;
-        if (c0 >= a.p_cols) return;
-        float ga[8], up[8];
+// Epilogue of a wave's block of 64 P rows and 16 NJ output rows, the first of them t0; col0
+// is its first output column.  Residuals are loaded two row blocks at a time, into the
+// registers that the fragments no longer need.
+template <class T, int LAYOUT, int EPI, int NJ>
+__device__ inline void finish(const LinearArgs& a, f32x4 (&acc)[4][NJ], int t0, int col0, int lane, int split) {
+    const int g = lane >> 4, c0 = col0 + g * (EPI == EPI_GATED ? 8 : 16);
+    ColumnTerms<T> col[2];
+    constexpr int AHEAD = NJ > 2 ? 2 : 1;
+    Resid8 resid[AHEAD][2];
+    if (!a.partial) {
+        col[0].load(a, c0, a.p_scale);
+        if constexpr (EPI == EPI_GATED) col[1].load(a, c0, a.p_scale ? a.p_scale + a.p_cols : nullptr);
+        else col[1].load(a, c0 + 8, a.p_scale);
+    }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            ga[e] = c[e >> 2][e & 3];
-            up[e] = c[2 + (e >> 2)][e & 3];
+    for (int j = 0; j < NJ; ++j) {
+        if (EPI == EPI_LINEAR && a.resid && j % AHEAD == 0) {
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    if (j + i < NJ) resid[i][h].load(a, t0 + (j + i) * 16 + (lane & 15), c0 + 8 * h);
         }
-        finish_gated8<T>(a, ga, up, t, c0, qs);
-    } else {
+        f32x4 c[4] = {acc[0][j], acc[1][j], acc[2][j], acc[3][j]};
+        if constexpr (LAYOUT != ROWS_ROWS) transpose_groups(c);
+        const long t = t0 + j * 16 + (lane & 15);
+        const float qs = T::bytes == 1 && a.q_scale ? a.q_scale[min(t, (long)a.q_rows - 1)] : 1.0f;
+        if (t < a.q_rows) {
+            if constexpr (EPI == EPI_GATED) {
+                float ga[8], up[8];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int c0 = col0 + g * 16 + h * 8;
-            if (c0 >= a.p_cols) return;
-            if (a.partial) {
-                float* o = a.partial + ((long)split * a.q_rows + t) * a.p_cols + c0;
-                *(f32x4*)o = c[2 * h];
-                *(f32x4*)(o + 4) = c[2 * h + 1];
+                for (int e = 0; e < 8; ++e) {
+                    ga[e] = c[e >> 2][e & 3];
+                    up[e] = c[2 + (e >> 2)][e & 3];
+                }
+                if (c0 < a.p_cols) finish_gated8<T>(a, ga, up, t, c0, qs, col[0], col[1]);
             } else {
-                float z[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) z[e] = c[2 * h + (e >> 2)][e & 3];
-                finish8<T>(a, z, t, c0, qs);
+                for (int h = 0; h < 2; ++h) {
+                    const int ch = c0 + 8 * h;
+                    if (ch >= a.p_cols) continue;
+                    if (a.partial) {
+                        float* o = a.partial + ((long)split * a.q_rows + t) * a.p_cols + ch;
+                        *(f32x4*)o = c[2 * h];
+                        *(f32x4*)(o + 4) = c[2 * h + 1];
+                    } else {
+                        float z[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) z[e] = c[2 * h + (e >> 2)][e & 3];
+                        finish8<T>(a, z, t, ch, qs, col[h], resid[j % AHEAD][h]);
+                    }
+                }
             }
         }
+        __builtin_amdgcn_sched_barrier(0);
     }
 }
 

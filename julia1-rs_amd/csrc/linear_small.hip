@@ -1,7 +1,7 @@
-// Linear and gated projections of few rows: W streams from memory straight into registers,
-// once per 16 * TB rows of X.  A workgroup of eight waves computes 16 * PT operand rows (PT =
-// 1 or 2 blocks of 16 columns; the gate and the up block of 16 columns when gated) for 16 * TB
-// rows of X; its waves take the K steps in turn and add their sums through LDS in wave order.
+// Linear and gated projections of up to 16 rows: W streams from memory straight into
+// registers, once.  A workgroup of eight waves computes 16 output columns (their gate and up
+// rows when gated); its waves take the K steps in turn, several loads in flight, and their sums
+// are added through LDS in wave order.
 #include <hip/hip_runtime.h>
 
 #include "linear.hpp"
@@ -12,35 +12,29 @@ namespace {
 
 constexpr int NW = 8;
 
-template <class T, int EPI, int PT, int TB>
+template <class T, int EPI>
 __global__ __launch_bounds__(64 * NW) void linear_small_kernel(LinearArgs a) {
-    constexpr int ES = T::bytes;
-    constexpr int PW = EPI == EPI_GATED ? 16 : 16 * PT;  // output columns of a workgroup
-    __shared__ __align__(16) f32x4 sums[NW][PT * TB][64];
+    constexpr int ES = T::bytes, PT = EPI == EPI_GATED ? 2 : 1;  // blocks of 16 P rows
+    __shared__ __align__(16) f32x4 sums[NW][PT][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, m = lane & 15;
-    const int p0 = blockIdx.x * PW, q0 = blockIdx.y * 16 * TB;
+    const int p0 = blockIdx.x * 16;
     const int kbytes = a.k * ES, steps = (kbytes + STEP_BYTES - 1) / STEP_BYTES;
 
     // Rows past the operand's end read its last row; those products are not stored.
-    const uint8_t *pr[PT], *qr[TB];
-#pragma unroll
-    for (int i = 0; i < PT; ++i) {
-        const long r = min(p0 + (EPI == EPI_GATED ? 0 : 16 * i) + m, a.p_cols - 1) + (EPI == EPI_GATED ? (long)i * a.p_cols : 0L);
-        pr[i] = (const uint8_t*)a.p + r * a.ldp * ES;
-    }
-#pragma unroll
-    for (int j = 0; j < TB; ++j) qr[j] = (const uint8_t*)a.q + (long)min(q0 + 16 * j + m, a.q_rows - 1) * a.ldq * ES;
-
-    f32x4 acc[PT][TB];
+    const uint8_t* pr[PT];
 #pragma unroll
     for (int i = 0; i < PT; ++i)
+        pr[i] = (const uint8_t*)a.p + (min(p0 + m, a.p_cols - 1) + (long)i * a.p_cols) * a.ldp * ES;
+    const uint8_t* const qr = (const uint8_t*)a.q + (long)min(m, a.q_rows - 1) * a.ldq * ES;
+
+    f32x4 acc[PT];
 #pragma unroll
-        for (int j = 0; j < TB; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+    for (int i = 0; i < PT; ++i) acc[i] = f32x4{0, 0, 0, 0};
 
     // Chunks past K are zeros in both operands (a NaN in either would spoil the sum).
-    constexpr int U = PT * TB <= 2 ? 4 : 2;  // K steps in flight per wave
+    constexpr int U = 4;  // K steps in flight per wave
     for (int s0 = wave; s0 < steps; s0 += NW * U) {
-        u32x4 pf[U][PT][2], qf[U][TB][2];
+        u32x4 pf[U][PT][2], qf[U][2];
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -53,80 +47,55 @@ __global__ __launch_bounds__(64 * NW) void linear_small_kernel(LinearArgs a) {
                     pf[u][i][h] = *(const u32x4*)(pr[i] + off);
                     if (!in) pf[u][i][h] = u32x4{0, 0, 0, 0};
                 }
-#pragma unroll
-                for (int j = 0; j < TB; ++j) {
-                    qf[u][j][h] = *(const u32x4*)(qr[j] + off);
-                    if (!in) qf[u][j][h] = u32x4{0, 0, 0, 0};
-                }
+                qf[u][h] = *(const u32x4*)(qr + off);
+                if (!in) qf[u][h] = u32x4{0, 0, 0, 0};
             }
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int i = 0; i < PT; ++i)
-#pragma unroll
-                for (int j = 0; j < TB; ++j)
-                    acc[i][j] = T::mfma(T::make(pf[u][i][0], pf[u][i][1]), T::make(qf[u][j][0], qf[u][j][1]), acc[i][j]);
+                acc[i] = T::mfma(T::make(pf[u][i][0], pf[u][i][1]), T::make(qf[u][0], qf[u][1]), acc[i]);
     }
 
+#pragma unroll
+    for (int i = 0; i < PT; ++i) sums[wave][i][lane] = acc[i];
+    __syncthreads();
+    // Eight columns of one row per thread: lanes of group g hold columns 4g .. 4g+3 of row
+    // lane % 16, so eight columns are two neighbouring groups.
+    const int row = threadIdx.x & 15, half = threadIdx.x >> 4, c0 = p0 + half * 8;
+    if (half > 1 || row >= a.q_rows || c0 >= a.p_cols) return;
+    const float qs = ES == 1 && a.q_scale ? a.q_scale[row] : 1.0f;
+    ColumnTerms<T> col[PT];
+    Resid8 resid;
+#pragma unroll
+    for (int i = 0; i < PT; ++i) col[i].load(a, c0, a.p_scale ? a.p_scale + (long)i * a.p_cols : nullptr);
+    if (a.resid) resid.load(a, row, c0);
+    float z[PT][8];
 #pragma unroll
     for (int i = 0; i < PT; ++i)
 #pragma unroll
-        for (int j = 0; j < TB; ++j) sums[wave][i * TB + j][lane] = acc[i][j];
-    __syncthreads();
-    // One output (row, 8 columns) per thread: lanes 0-15 of group g hold columns 4g .. 4g+3,
-    // so 8 columns are two neighbouring groups.
-    constexpr int BLOCKS = EPI == EPI_GATED ? TB : PT * TB;
-    for (int o = threadIdx.x; o < BLOCKS * 32; o += 64 * NW) {
-        const int blk = o >> 5, half = (o >> 4) & 1, row = o & 15;
-        const int j = blk % TB, i = blk / TB;
-        const long t = q0 + 16 * j + row;
-        const int c0 = p0 + 16 * i + half * 8;
-        if (t >= a.q_rows || c0 >= a.p_cols) continue;
-        auto total = [&](int tile, float (&v)[8]) {
+        for (int h = 0; h < 2; ++h) {
+            const int l = (half * 2 + h) * 16 + row;
+            f32x4 s = sums[0][i][l];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int l = (half * 2 + h) * 16 + row;
-                f32x4 s = sums[0][tile][l];
+            for (int w = 1; w < NW; ++w) s += sums[w][i][l];
 #pragma unroll
-                for (int w = 1; w < NW; ++w) s += sums[w][tile][l];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[4 * h + e] = s[e];
-            }
-        };
-        const float qs = ES == 1 && a.q_scale ? a.q_scale[t] : 1.0f;
-        if constexpr (EPI == EPI_GATED) {
-            float ga[8], up[8];
-            total(j, ga);
-            total(TB + j, up);
-            finish_gated8<T>(a, ga, up, t, c0, qs);
-        } else {
-            float z[8];
-            total(i * TB + j, z);
-            finish8<T>(a, z, t, c0, qs);
+            for (int e = 0; e < 4; ++e) z[i][4 * h + e] = s[e];
         }
-    }
+    if constexpr (EPI == EPI_GATED) finish_gated8<T>(a, z[0], z[1], row, c0, qs, col[0], col[1]);
+    else finish8<T>(a, z[0], row, c0, qs, col[0], resid);
 }
 
-template <class T, int EPI, int PT, int TB>
+template <class T, int EPI>
 void launch(const LinearArgs& a, hipStream_t s) {
-    const unsigned pw = EPI == EPI_GATED ? 16 : 16 * PT;
-    JH_LAUNCH((linear_small_kernel<T, EPI, PT, TB>),
-              dim3((unsigned)(a.p_cols + pw - 1) / pw, (unsigned)(a.q_rows + 16 * TB - 1) / (16 * TB)), dim3(64 * NW), 0,
-              s, a);
+    JH_LAUNCH((linear_small_kernel<T, EPI>), dim3((unsigned)(a.p_cols + 15) / 16), dim3(64 * NW), 0, s, a);
     HIP_CHECK(hipGetLastError());
 }
 
 template <class T>
 void dispatch(const LinearArgs& a, hipStream_t s) {
-    if (a.gated) {
-        if (a.q_rows <= 16) launch<T, EPI_GATED, 2, 1>(a, s);
-        else if (a.q_rows <= 32) launch<T, EPI_GATED, 2, 2>(a, s);
-        else launch<T, EPI_GATED, 2, 4>(a, s);
-    } else {
-        if (a.q_rows <= 16) launch<T, EPI_LINEAR, 1, 1>(a, s);
-        else if (a.q_rows <= 32) launch<T, EPI_LINEAR, 2, 2>(a, s);
-        else launch<T, EPI_LINEAR, 2, 4>(a, s);
-    }
+    if (a.gated) launch<T, EPI_GATED>(a, s);
+    else launch<T, EPI_LINEAR>(a, s);
 }
 
 }  // namespace

@@ -356,17 +356,32 @@ __global__ __launch_bounds__(THREADS) void rms_norm_backward_kernel(RmsNormGradA
     }
 }
 
-// out[c] = sum over r of in[r, c], FP32 parts in row order: a workgroup owns 64 columns,
-// wave w adds rows w, w + 4, ... and the four sums are added in wave order.
-__global__ __launch_bounds__(THREADS) void column_sum_kernel(const float* in, int rows, int cols, float* out) {
-    __shared__ float part[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
-    float s = 0.0f;
-    if (c < cols)
-        for (int r = wave; r < rows; r += 4) s += in[(long)r * cols + c];
-    part[wave][lane] = s;
+// out[c] = sum over r of in[r, c] in FP32: a workgroup owns 64 columns, four per lane of 16,
+// and its 64 groups of 16 lanes each add a run of rows, eight loads in flight; the groups' sums
+// are added in group order.
+constexpr int SUM_THREADS = 1024, SUM_GROUPS = SUM_THREADS / 16;
+__global__ __launch_bounds__(SUM_THREADS) void column_sum_kernel(const float* in, int rows, int cols, float* out) {
+    __shared__ __align__(16) float part[SUM_GROUPS][64];
+    const int lane = threadIdx.x & 15, grp = threadIdx.x >> 4, c = blockIdx.x * 64 + lane * 4;
+    const int per = (rows + SUM_GROUPS - 1) / SUM_GROUPS, r0 = grp * per, r1 = min(rows, r0 + per);
+    f32x4 s = {0, 0, 0, 0};
+    if (c < cols) {
+        for (int r = r0; r < r1; r += 8) {
+            f32x4 v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = *(const f32x4*)(in + (long)min(r + i, r1 - 1) * cols + c);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (r + i < r1) s += v[i];
+        }
+    }
+    *(f32x4*)&part[grp][lane * 4] = s;
     __syncthreads();
-    if (wave == 0 && c < cols) out[c] = ((part[0][lane] + part[1][lane]) + part[2][lane]) + part[3][lane];
+    if (threadIdx.x < 64 && blockIdx.x * 64 + threadIdx.x < cols) {
+        float t = 0.0f;
+        for (int g = 0; g < SUM_GROUPS; ++g) t += part[g][threadIdx.x];
+        out[blockIdx.x * 64 + threadIdx.x] = t;
+    }
 }
 
 // f<TPR, NC>() for the number of 8-value chunks each of a row's threads holds.
@@ -568,6 +583,6 @@ void rms_norm_backward(const RmsNormGradArgs& args, size_t workspace_bytes, hipS
 }
 
 void launch_column_sum(const float* in, int rows, int cols, float* out, hipStream_t s) {
-    JH_LAUNCH(column_sum_kernel, dim3((unsigned)(cols + 63) / 64), dim3(THREADS), 0, s, in, rows, cols, out);
+    JH_LAUNCH(column_sum_kernel, dim3((unsigned)(cols + 63) / 64), dim3(SUM_THREADS), 0, s, in, rows, cols, out);
     HIP_CHECK(hipGetLastError());
 }

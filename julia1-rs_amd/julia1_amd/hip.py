@@ -350,89 +350,105 @@ def op_attention(q, ldq, k, v, ldkv, out, ldo, tiles, heads, window, scale=0.125
 
 ACTS = {"none": abi.ACT_NONE, "relu": abi.ACT_RELU, "gelu": abi.ACT_GELU, "gelu_tanh": abi.ACT_GELU_TANH,
         "silu": abi.ACT_SILU}
-_TYPES = None
-
-
-def _type(t):
-    """The element type code of a torch tensor."""
-    global _TYPES
-    if _TYPES is None:
-        import torch
-        _TYPES = {torch.float32: abi.F32, torch.bfloat16: abi.BF16, torch.float16: abi.F16,
-                  torch.float8_e4m3fn: abi.E4M3}
-    code = _TYPES.get(t.dtype)
-    if code is None:
-        raise HipError(abi.JH_ERR_INVALID, f"no such element type: {t.dtype}")
-    return code
+_TYPES = {}
 
 
 def _invalid(msg):
     raise HipError(abi.JH_ERR_INVALID, msg)
 
 
-def _mat(name, t, rows, cols, dev, dtype=None):
+def _type(t):
+    """The element type code of a torch tensor."""
+    code = _TYPES.get(t.dtype)
+    if code is None:
+        import torch
+        _TYPES.update({torch.float32: abi.F32, torch.bfloat16: abi.BF16, torch.float16: abi.F16,
+                       torch.float8_e4m3fn: abi.E4M3})
+        code = _TYPES.get(t.dtype)
+        if code is None:
+            _invalid(f"no such element type: {t.dtype}")
+    return code
+
+
+def _mat(name, t, shape, dev, dtype=None):
     """(address, row stride) of a 2-D tensor of the wanted shape, device and type; (None, 0) for None."""
     if t is None:
         return None, 0
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
-        _invalid(f"{name}: shape {tuple(t.shape)}, expected {(rows, cols)}")
-    ld = t.stride(0)
-    if (cols > 1 and t.stride(1) != 1) or ld < 0 or t.device != dev:
-        _invalid(f"{name}: needs contiguous rows on {dev}")
-    if dtype is not None and t.dtype != dtype:
-        _invalid(f"{name}: {t.dtype}, expected {dtype}")
-    return t.data_ptr(), max(ld, cols) if rows <= 1 else ld
+    if t.shape != shape or t.get_device() != dev or (dtype is not None and t.dtype is not dtype):
+        _invalid(f"{name}: {t.dtype} {tuple(t.shape)} on {t.device}, expected {dtype or 'a matrix'} {tuple(shape)} "
+                 "on the first operand's device")
+    ld, one = t.stride()
+    if one != 1 and shape[1] > 1:
+        _invalid(f"{name}: needs contiguous rows")
+    return t.data_ptr(), ld
 
 
 def _vec(name, t, n, dev):
     """Address of a contiguous f32 vector of n values; None for None."""
     if t is None:
         return None
-    import torch
-    if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous() or t.device != dev:
-        _invalid(f"{name}: needs {n} contiguous float32 values on {dev}")
+    if _type(t) != abi.F32 or t.numel() != n or not t.is_contiguous() or t.get_device() != dev:
+        _invalid(f"{name}: needs {n} contiguous float32 values on the first operand's device")
     return t.data_ptr()
 
 
-def _weight(name, t, rows, cols, dev, dtype):
+def _weight(name, t, shape, dev, dtype=None):
     if t is not None and not t.is_contiguous():
         _invalid(f"{name}: needs a contiguous matrix")
-    return _mat(name, t, rows, cols, dev, dtype)[0]
+    return _mat(name, t, shape, dev, dtype)[0]
 
 
 def _space(t, dev):
     if t is None:
         return None, 0
-    if not t.is_contiguous() or t.device != dev:
-        _invalid(f"workspace: needs contiguous memory on {dev}")
+    if not t.is_contiguous() or t.get_device() != dev:
+        _invalid("workspace: needs contiguous memory on the first operand's device")
     return t.data_ptr(), t.numel() * t.element_size()
 
 
 def _act(name):
-    if name not in ACTS:
+    code = ACTS.get(name)
+    if code is None:
         _invalid(f"unknown activation {name!r}")
-    return ACTS[name]
+    return code
+
+
+def _bytes(n):
+    if lib().jh_last_error():
+        raise HipError(abi.JH_ERR_INVALID, lib().jh_last_error().decode())
+    return n
+
+
+def _two_d(name, t):
+    if t.dim() != 2:
+        _invalid(f"{name}: needs a matrix")
+    return t.shape
 
 
 def op_rms_norm(x, w, eps, out, resid=None, resid_out=None, scales=None, rstd=None, stream=None):
     """jh_op_rms_norm: out = RMS norm of s = x + resid, times w; s goes to resid_out (which may be resid).  out of
     torch.float8_e4m3fn takes e4m3 codes and scales their f32 scale per row; rstd (f32) is kept for the backward."""
-    (rows, h), dev = x.shape, x.device
-    (xp, ldx), (op, ldo) = _mat("x", x, rows, h, dev), _mat("out", out, rows, h, dev)
-    rp, ldr = _mat("resid", resid, rows, h, dev)
-    sp, lds = _mat("resid_out", resid_out, rows, h, dev, None if resid is None else resid.dtype)
-    check(lib().jh_op_rms_norm(_type(x), xp, ldx, 0 if resid is None else _type(resid), rp, ldr, sp, lds, rows, h,
-                               _vec("w", w, h, dev), eps, _type(out), op, ldo, _vec("scales", scales, rows, dev),
-                               _vec("rstd", rstd, rows, dev), stream))
+    shape, dev = _two_d("x", x), x.get_device()
+    rows, h = shape
+    xp, ldx = _mat("x", x, shape, dev)
+    op, ldo = _mat("out", out, shape, dev)
+    rp = sp = None
+    rt = ldr = lds = 0
+    if resid is not None or resid_out is not None:
+        rt = _type(resid_out if resid is None else resid)
+        rp, ldr = _mat("resid", resid, shape, dev)
+        sp, lds = _mat("resid_out", resid_out, shape, dev, None if resid is None else resid.dtype)
+    check(lib().jh_op_rms_norm(_type(x), xp, ldx, rt, rp, ldr, sp, lds, rows, h, _vec("w", w, h, dev), eps, _type(out),
+                               op, ldo, _vec("scales", scales, rows, dev), _vec("rstd", rstd, rows, dev), stream))
 
 
 def op_rms_norm_backward(dy, s, w, rstd, ds, dw=None, workspace=None, dres=None, stream=None):
     """jh_op_rms_norm_backward: ds (+ dres) and dw from dy, with s = resid_out (or x) and rstd of op_rms_norm; dw
     needs a workspace tensor of rms_norm_backward_workspace(rows, hidden) bytes."""
-    (rows, h), dev = dy.shape, dy.device
-    (yp, ldy), (sp, lds) = _mat("dy", dy, rows, h, dev), _mat("s", s, rows, h, dev)
-    dp, ldd = _mat("ds", ds, rows, h, dev)
-    rp, ldr = _mat("dres", dres, rows, h, dev, ds.dtype)
+    shape, dev = _two_d("dy", dy), dy.get_device()
+    rows, h = shape
+    (yp, ldy), (sp, lds), (dp, ldd) = _mat("dy", dy, shape, dev), _mat("s", s, shape, dev), _mat("ds", ds, shape, dev)
+    rp, ldr = _mat("dres", dres, shape, dev, ds.dtype)
     wp, wb = _space(workspace, dev)
     check(lib().jh_op_rms_norm_backward(_type(dy), yp, ldy, _type(s), sp, lds, rows, h, _vec("w", w, h, dev),
                                         _vec("rstd", rstd, rows, dev), _type(ds), rp, ldr, dp, ldd,
@@ -443,43 +459,44 @@ def rms_norm_backward_workspace(rows, hidden) -> int:
     return _bytes(lib().jh_op_rms_norm_backward_workspace(rows, hidden))
 
 
-def _bytes(n):
-    if lib().jh_last_error():
-        raise HipError(abi.JH_ERR_INVALID, lib().jh_last_error().decode())
-    return n
-
-
 def op_quantize_rows(x, q, scales, stream=None):
     """jh_op_quantize_rows: e4m3 codes q (torch.float8_e4m3fn) of x's rows and their f32 scales."""
-    import torch
-    (rows, n), dev = x.shape, x.device
-    (xp, ldx), (qp, ldq) = _mat("x", x, rows, n, dev), _mat("q", q, rows, n, dev, torch.float8_e4m3fn)
+    shape, dev = _two_d("x", x), x.get_device()
+    rows, n = shape
+    (xp, ldx), (qp, ldq) = _mat("x", x, shape, dev), _mat("q", q, shape, dev)
+    if _type(q) != abi.E4M3:
+        _invalid("q: needs torch.float8_e4m3fn")
     check(lib().jh_op_quantize_rows(_type(x), xp, ldx, rows, n, qp, ldq, _vec("scales", scales, rows, dev), stream))
 
 
 def op_linear(x, w, out, bias=None, act="none", resid=None, x_scale=None, w_scale=None, pre=None, stream=None):
     """jh_op_linear: out = act(x w^T + bias) + resid; x and w of one type (bf16, f16, or float8_e4m3fn with x_scale and
     w_scale), out f32 or their type (bf16 for e4m3); resid may be out; pre keeps x w^T + bias for the backward."""
-    (rows, k), dev = x.shape, x.device
-    n = w.shape[0]
-    (xp, ldx), (op, ldo) = _mat("x", x, rows, k, dev), _mat("out", out, rows, n, dev)
-    (rp, ldr), (pp, ldp) = _mat("resid", resid, rows, n, dev, out.dtype), _mat("pre", pre, rows, n, dev, x.dtype)
+    rows, k = _two_d("x", x)
+    n, dev, dt = w.shape[0], x.get_device(), x.dtype
+    shape = (rows, n)
+    xp, ldx = _mat("x", x, x.shape, dev)
+    op, ldo = _mat("out", out, shape, dev)
+    rp, ldr = (None, 0) if resid is None else _mat("resid", resid, shape, dev, out.dtype)
+    pp, ldp = (None, 0) if pre is None else _mat("pre", pre, shape, dev, dt)
     check(lib().jh_op_linear(_type(x), xp, ldx, _vec("x_scale", x_scale, rows, dev), rows,
-                             _weight("w", w, n, k, dev, x.dtype), _vec("w_scale", w_scale, n, dev), n, k,
+                             _weight("w", w, (n, k), dev, dt), _vec("w_scale", w_scale, n, dev), n, k,
                              _vec("bias", bias, n, dev), _act(act), rp, ldr, _type(out), op, ldo, pp, ldp, stream))
 
 
 def op_linear_backward(dy, x, w, workspace, act="none", pre=None, dx=None, dw=None, dbias=None, stream=None):
     """jh_op_linear_backward: whichever of dx, dw (f32 or x's type) and dbias (f32) are given, from dy and (act not
     "none") pre; workspace of linear_backward_workspace(rows, n, k, act) bytes."""
-    (rows, n), dev = dy.shape, dy.device
+    shape, dev, dt = _two_d("dy", dy), dy.get_device(), dy.dtype
+    rows, n = shape
     k = w.shape[1]
-    (yp, ldy), (xp, ldx) = _mat("dy", dy, rows, n, dev), _mat("x", x, rows, k, dev, dy.dtype)
-    (pp, ldp), (dp, ldd) = _mat("pre", pre, rows, n, dev, dy.dtype), _mat("dx", dx, rows, k, dev, dy.dtype)
+    yp, ldy = _mat("dy", dy, shape, dev)
+    (xp, ldx), (dp, ldd) = _mat("x", x, (rows, k), dev, dt), _mat("dx", dx, (rows, k), dev, dt)
+    pp, ldp = _mat("pre", pre, shape, dev, dt)
     wp, wb = _space(workspace, dev)
-    check(lib().jh_op_linear_backward(_type(dy), yp, ldy, xp, ldx, rows, _weight("w", w, n, k, dev, dy.dtype), n, k,
+    check(lib().jh_op_linear_backward(_type(dy), yp, ldy, xp, ldx, rows, _weight("w", w, (n, k), dev, dt), n, k,
                                       _act(act), pp, ldp, dp, ldd, _type(dy if dw is None else dw),
-                                      _weight("dw", dw, n, k, dev, None), _vec("dbias", dbias, n, dev), wp, wb, stream))
+                                      _weight("dw", dw, (n, k), dev), _vec("dbias", dbias, n, dev), wp, wb, stream))
 
 
 def linear_backward_workspace(rows, n, k, act="none") -> int:
@@ -489,32 +506,32 @@ def linear_backward_workspace(rows, n, k, act="none") -> int:
 def op_gated_ffn(x, wi, out, act="gelu", x_scale=None, w_scale=None, gu=None, stream=None):
     """jh_op_gated_ffn: out = act(x Wg^T) * (x Wu^T), wi = [Wg; Wu]; types as op_linear (out of x's type, bf16 for
     e4m3); gu [rows, 2 inter] keeps both projections for the backward."""
-    (rows, k), dev = x.shape, x.device
-    n = wi.shape[0]
+    rows, k = _two_d("x", x)
+    n, dev, dt, code = wi.shape[0], x.get_device(), x.dtype, _type(x)
     if n % 2:
         _invalid("wi: needs an even number of rows")
-    half = None if _type(x) == abi.E4M3 else x.dtype
-    (xp, ldx), (op, ldo) = _mat("x", x, rows, k, dev), _mat("out", out, rows, n // 2, dev, half)
-    if half is None and _type(out) != abi.BF16:
-        _invalid("out: e4m3 operands give bfloat16")
-    gp, ldg = _mat("gu", gu, rows, n, dev, x.dtype)
-    check(lib().jh_op_gated_ffn(_type(x), xp, ldx, _vec("x_scale", x_scale, rows, dev), rows,
-                                _weight("wi", wi, n, k, dev, x.dtype), _vec("w_scale", w_scale, n, dev), n // 2, k,
+    if _type(out) != (abi.BF16 if code == abi.E4M3 else code):
+        _invalid("out: has x's type (bfloat16 for e4m3)")
+    xp, ldx = _mat("x", x, x.shape, dev)
+    op, ldo = _mat("out", out, (rows, n // 2), dev)
+    gp, ldg = (None, 0) if gu is None else _mat("gu", gu, (rows, n), dev, dt)
+    check(lib().jh_op_gated_ffn(code, xp, ldx, _vec("x_scale", x_scale, rows, dev), rows,
+                                _weight("wi", wi, (n, k), dev, dt), _vec("w_scale", w_scale, n, dev), n // 2, k,
                                 _act(act), op, ldo, gp, ldg, stream))
 
 
 def op_gated_ffn_backward(dh, gu, x, wi, workspace, act="gelu", dx=None, dw=None, stream=None):
     """jh_op_gated_ffn_backward: dx and / or dw (of wi; f32 or x's type) from dh and gu; workspace of
     gated_ffn_backward_workspace(rows, inter, k) bytes."""
-    (rows, inter), dev = dh.shape, dh.device
-    k = wi.shape[1]
-    (hp, ldh), (gp, ldg) = _mat("dh", dh, rows, inter, dev), _mat("gu", gu, rows, 2 * inter, dev, dh.dtype)
-    (xp, ldx), (dp, ldd) = _mat("x", x, rows, k, dev, dh.dtype), _mat("dx", dx, rows, k, dev, dh.dtype)
+    shape, dev, dt = _two_d("dh", dh), dh.get_device(), dh.dtype
+    rows, inter = shape
+    k, n = wi.shape[1], 2 * inter
+    (hp, ldh), (gp, ldg) = _mat("dh", dh, shape, dev), _mat("gu", gu, (rows, n), dev, dt)
+    (xp, ldx), (dp, ldd) = _mat("x", x, (rows, k), dev, dt), _mat("dx", dx, (rows, k), dev, dt)
     wp, wb = _space(workspace, dev)
-    check(lib().jh_op_gated_ffn_backward(_type(dh), hp, ldh, gp, ldg, xp, ldx, rows,
-                                         _weight("wi", wi, 2 * inter, k, dev, dh.dtype), inter, k, _act(act), dp, ldd,
-                                         _type(dh if dw is None else dw), _weight("dw", dw, 2 * inter, k, dev, None),
-                                         wp, wb, stream))
+    check(lib().jh_op_gated_ffn_backward(_type(dh), hp, ldh, gp, ldg, xp, ldx, rows, _weight("wi", wi, (n, k), dev, dt),
+                                         inter, k, _act(act), dp, ldd, _type(dh if dw is None else dw),
+                                         _weight("dw", dw, (n, k), dev), wp, wb, stream))
 
 
 def gated_ffn_backward_workspace(rows, inter, k) -> int:
