@@ -197,14 +197,14 @@ double cost(int kernel, const LinearArgs& a, long splits) {
 struct Choice {
     int kernel;
     int splits;
+    double cost;
 };
 
 // The cheapest kernel and, for gradients, number of parts of the contraction, whose FP32 sums
 // take `splits` outputs' worth of memory (at most 16, and 48 MiB) and one more kernel.
 constexpr long MAX_SPLITS = 16, SPLIT_BYTES = 48L << 20, MIN_STEPS = 4;
 Choice pick(const LinearArgs& a, bool gradient) {
-    Choice best{PAIR, 1};
-    double least = 1e30;
+    Choice best{PAIR, 1, 1e30};
     const double out = (double)a.q_rows * a.p_cols * 4;
     for (long splits = 1; splits <= (gradient ? MAX_SPLITS : 1); splits += splits < 4 ? 1 : splits < 8 ? 2 : 4) {
         if (splits > 1 && (steps_of(a) < splits * MIN_STEPS || out * splits > SPLIT_BYTES)) break;
@@ -212,13 +212,36 @@ Choice pick(const LinearArgs& a, bool gradient) {
         for (int kernel = 0; kernel < KERNELS; ++kernel) {
             if (kernel == WIDE && a.type == JH_E4M3 && a.out_f32) continue;  // has no bf16 fragments of e4m3
             const double c = cost(kernel, a, splits) + sum;
-            if (c < least) {
-                least = c;
-                best = {kernel, (int)splits};
-            }
+            if (c < best.cost) best = {kernel, (int)splits, c};
         }
     }
     return best;
+}
+
+// Output rows [r0, r0 + rows) of a product.
+LinearArgs row_range(const LinearArgs& a, int r0, int rows) {
+    LinearArgs r = a;
+    const long es = a.type == JH_E4M3 ? 1 : 2, os = a.out_f32 ? 4 : 2;
+    r.q = (const uint8_t*)a.q + (a.layout == COLS_COLS ? r0 : r0 * a.ldq) * es;
+    r.q_rows = rows;
+    if (a.q_scale) r.q_scale = a.q_scale + r0;
+    if (a.resid) r.resid = (const uint8_t*)a.resid + r0 * a.ldr * os;
+    r.out = (uint8_t*)a.out + r0 * a.ldo * os;
+    if (a.pre) r.pre = (uint8_t*)a.pre + r0 * a.ldpre * 2;
+    return r;
+}
+
+// Rows that 256 x 256 tiles take in whole rounds of the CUs, where that and another kernel
+// for the rest come cheaper than any kernel alone; else 0.  9482 x 4096 x 1024 (608 tiles, 2.4
+// rounds): 7936 rows in two rounds, the rest in one of 128 x 128 tiles.
+int whole_rounds(const LinearArgs& a, double alone) {
+    if (a.type == JH_E4M3 && a.out_f32) return 0;
+    const long across = tiles_of(row_range(a, 0, 1), 256, 256), rounds = tiles_of(a, 256, 256) / (long)CUS;
+    const long rows = rounds * (long)CUS / across * 256;
+    if (rows <= 0 || rows >= a.q_rows) return 0;
+    const double c = cost(WIDE, row_range(a, 0, (int)rows), 1) +
+                     pick(row_range(a, (int)rows, a.q_rows - (int)rows), false).cost;
+    return c < alone ? (int)rows : 0;
 }
 
 long partial_bytes(const LinearArgs& a) {
@@ -244,11 +267,21 @@ void split_sum(const LinearArgs& a, hipStream_t s) {
 // tiles; 17 to 32 rows, two blocks of them, took 18.2 against 17.6).
 constexpr int STREAM_ROWS = 16;
 
+void run_whole(const LinearArgs& a, const Choice& c, hipStream_t s) {
+    if (const int rows = whole_rounds(a, c.cost)) {
+        const LinearArgs rest = row_range(a, rows, a.q_rows - rows);
+        launch(WIDE, row_range(a, 0, rows), s);
+        launch(pick(rest, false).kernel, rest, s);
+    } else {
+        launch(c.kernel, a, s);
+    }
+}
+
 void run(LinearArgs a, hipStream_t s) {
     a.splits = 1;
     a.split_steps = 0x7fffffff;
     if (a.q_rows <= STREAM_ROWS) launch_linear_small(a, s);
-    else launch(pick(a, false).kernel, a, s);
+    else run_whole(a, pick(a, false), s);
 }
 
 // A gradient product, its contraction split where that fills the GPU.
@@ -258,8 +291,8 @@ void run_gradient(LinearArgs a, float* partial, hipStream_t s) {
     a.split_steps = (int)((steps_of(a) + c.splits - 1) / c.splits);
     a.splits = c.splits;
     a.partial = c.splits > 1 ? partial : nullptr;
+    if (c.splits == 1) return run_whole(a, c, s);
     launch(c.kernel, a, s);
-    if (c.splits == 1) return;
     if (a.type == JH_BF16) split_sum<Bf16>(a, s);
     else split_sum<F16>(a, s);
 }

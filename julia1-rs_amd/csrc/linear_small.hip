@@ -1,6 +1,6 @@
 // Linear and gated projections of up to 16 rows: W streams from memory straight into
 // registers, once.  A workgroup of eight waves computes 16 output columns (their gate and up
-// rows when gated); its waves take the K steps in turn, several loads in flight, and their sums
+// rows when gated); its waves take pieces of K in turn, several loads in flight, and their sums
 // are added through LDS in wave order.
 #include <hip/hip_runtime.h>
 
@@ -18,7 +18,7 @@ __global__ __launch_bounds__(64 * NW) void linear_small_kernel(LinearArgs a) {
     __shared__ __align__(16) f32x4 sums[NW][PT][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, m = lane & 15;
     const int p0 = blockIdx.x * 16;
-    const int kbytes = a.k * ES, steps = (kbytes + STEP_BYTES - 1) / STEP_BYTES;
+    const int kbytes = a.k * ES, pieces = (kbytes + 63) / 64;
 
     // Rows past the operand's end read its last row; those products are not stored.
     const uint8_t* pr[PT];
@@ -31,30 +31,29 @@ __global__ __launch_bounds__(64 * NW) void linear_small_kernel(LinearArgs a) {
 #pragma unroll
     for (int i = 0; i < PT; ++i) acc[i] = f32x4{0, 0, 0, 0};
 
-    // Chunks past K are zeros in both operands (a NaN in either would spoil the sum).
-    constexpr int U = 4;  // K steps in flight per wave
-    for (int s0 = wave; s0 < steps; s0 += NW * U) {
-        u32x4 pf[U][PT][2], qf[U][2];
+    // 64 bytes of every row at a time, which the waves take in turn; chunks past K are zeros in
+    // both operands (a NaN in either would spoil the sum).
+    constexpr int U = 8;  // loads of each row in flight per wave
+    const u32x4 zero = {0, 0, 0, 0};
+    for (int s0 = wave; s0 < pieces; s0 += NW * U) {
+        u32x4 pf[U][PT], qf[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; ++u) {
+            const int at = (s0 + u * NW) * 64 + g * 16;
+            qf[u] = zero;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int at = (s0 + u * NW) * STEP_BYTES + h * 64 + g * 16;
-                const bool in = at < kbytes;
-                const int off = in ? at : 0;
+            for (int i = 0; i < PT; ++i) pf[u][i] = zero;
+            if (at < kbytes) {
 #pragma unroll
-                for (int i = 0; i < PT; ++i) {
-                    pf[u][i][h] = *(const u32x4*)(pr[i] + off);
-                    if (!in) pf[u][i][h] = u32x4{0, 0, 0, 0};
-                }
-                qf[u][h] = *(const u32x4*)(qr + off);
-                if (!in) qf[u][h] = u32x4{0, 0, 0, 0};
+                for (int i = 0; i < PT; ++i) pf[u][i] = *(const u32x4*)(pr[i] + at);
+                qf[u] = *(const u32x4*)(qr + at);
             }
+        }
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; u += 2)
 #pragma unroll
             for (int i = 0; i < PT; ++i)
-                acc[i] = T::mfma(T::make(pf[u][i][0], pf[u][i][1]), T::make(qf[u][0], qf[u][1]), acc[i]);
+                acc[i] = T::mfma(T::make(pf[u][i], pf[u + 1][i]), T::make(qf[u], qf[u + 1]), acc[i]);
     }
 
 #pragma unroll

@@ -149,6 +149,30 @@ __device__ inline u32x2 e4m3_codes(const double (&p)[8], double a, double inv) {
     return u32x2{h[0] | h[1] << 16, h[2] | h[3] << 16};
 }
 
+// The same for values of 16 bits, in 32: 448 p has 14 bits at most, so n is exact.  q1 is the
+// correctly rounded quotient of n by a (a product with the reciprocal, corrected once), and the
+// sign of its remainder, exact too, says on which side of q1 the quotient itself lies.  That
+// makes the float rounded to odd.  `lift` (a power of two) keeps the remainder
+// normal and n finite where the row's maximum is far from 1.  (9482 x 1152 bf16: 12.7 us in 64
+// bits, bound by arithmetic.)
+__device__ inline u32x2 e4m3_codes_half(const float (&p)[8], float a, float inv, float lift) {
+    uint32_t h[4];
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+        float q[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float n = p[e + i] * (E4M3_MAX * lift), q0 = n * inv;
+            const float q1 = __builtin_fmaf(__builtin_fmaf(-q0, a, n), inv, q0), r = __builtin_fmaf(-q1, a, n);
+            const int u = __builtin_bit_cast(int, q1), away = (__builtin_bit_cast(int, r) ^ u) >> 31;
+            // a NaN compares unequal and stays one
+            q[i] = __builtin_bit_cast(float, r == 0.0f ? u : (u + away) | 1);
+        }
+        h[e >> 1] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false) & 0xffffu;
+    }
+    return u32x2{h[0] | h[1] << 16, h[2] | h[3] << 16};
+}
+
 // One row per TPR threads; NC chunks of 8 values per thread.
 template <int TPR>
 __device__ inline bool row_of(int rows, long& row, int& lane) {
@@ -251,8 +275,18 @@ __global__ __launch_bounds__(THREADS) void quantize_rows_kernel(RmsNormArgs a) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(v[c][e]));
     m = row_max<TPR>(m, max_slot);
-    const double inv = m > 0.0f ? 1.0 / (double)m : 0.0;
     if (lane == 0) a.scales[row] = m / E4M3_MAX;
+    if constexpr (Elem<TX>::bytes == 2) {
+        const float lift = m < 0x1p-40f ? 0x1p96f : m > 0x1p100f ? 0x1p-64f : 1.0f;
+        const float top = m * lift, inv = m > 0.0f ? 1.0f / top : 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int i = (c * TPR + lane) * 8;
+            if (i < a.hidden) *(u32x2*)((uint8_t*)a.out + row * a.ldo + i) = e4m3_codes_half(v[c], top, inv, lift);
+        }
+        return;
+    }
+    const double inv = m > 0.0f ? 1.0 / (double)m : 0.0;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         const int i = (c * TPR + lane) * 8;

@@ -370,32 +370,49 @@ def _type(t):
     return code
 
 
-def _mat(name, t, shape, dev, dtype=None):
-    """(address, row stride) of a 2-D tensor of the wanted shape, device and type; (None, 0) for None."""
-    if t is None:
-        return None, 0
-    if t.shape != shape or t.get_device() != dev or (dtype is not None and t.dtype is not dtype):
-        _invalid(f"{name}: {t.dtype} {tuple(t.shape)} on {t.device}, expected {dtype or 'a matrix'} {tuple(shape)} "
-                 "on the first operand's device")
+# These run before every launch of a few microseconds, so they ask a tensor for no more than they need.
+
+def _first(name, t):
+    """(address, row stride, shape, device) of an operator's first operand, a 2-D tensor."""
+    shape = t.shape
+    if len(shape) != 2:
+        _invalid(f"{name}: needs a matrix")
     ld, one = t.stride()
     if one != 1 and shape[1] > 1:
         _invalid(f"{name}: needs contiguous rows")
-    return t.data_ptr(), ld
+    return t.data_ptr(), ld, shape, t.get_device()
+
+
+def _mat(name, t, shape, dev, dtype):
+    """(address, row stride) of a 2-D tensor of the wanted shape, type and device; (None, 0) for None."""
+    if t is None:
+        return None, 0
+    if t.shape == shape and t.dtype is dtype and t.get_device() == dev:
+        ld, one = t.stride()
+        if one == 1 or shape[1] <= 1:
+            return t.data_ptr(), ld
+        _invalid(f"{name}: needs contiguous rows")
+    _invalid(f"{name}: {t.dtype} {tuple(t.shape)} on {t.device}, expected {dtype} {tuple(shape)} on the first operand's "
+             "device")
+
+
+def _weight(name, t, shape, dev, dtype):
+    """Address of a contiguous matrix; None for None."""
+    if t is None:
+        return None
+    if t.shape == shape and t.dtype is dtype and t.get_device() == dev and t.is_contiguous():
+        return t.data_ptr()
+    _invalid(f"{name}: {t.dtype} {tuple(t.shape)} on {t.device}, expected contiguous {dtype} {tuple(shape)} on the first "
+             "operand's device")
 
 
 def _vec(name, t, n, dev):
     """Address of a contiguous f32 vector of n values; None for None."""
     if t is None:
         return None
-    if _type(t) != abi.F32 or t.numel() != n or not t.is_contiguous() or t.get_device() != dev:
-        _invalid(f"{name}: needs {n} contiguous float32 values on the first operand's device")
-    return t.data_ptr()
-
-
-def _weight(name, t, shape, dev, dtype=None):
-    if t is not None and not t.is_contiguous():
-        _invalid(f"{name}: needs a contiguous matrix")
-    return _mat(name, t, shape, dev, dtype)[0]
+    if t.numel() == n and _type(t) == abi.F32 and t.is_contiguous() and t.get_device() == dev:
+        return t.data_ptr()
+    _invalid(f"{name}: needs {n} contiguous float32 values on the first operand's device")
 
 
 def _space(t, dev):
@@ -419,35 +436,33 @@ def _bytes(n):
     return n
 
 
-def _two_d(name, t):
-    if t.dim() != 2:
-        _invalid(f"{name}: needs a matrix")
-    return t.shape
-
-
 def op_rms_norm(x, w, eps, out, resid=None, resid_out=None, scales=None, rstd=None, stream=None):
     """jh_op_rms_norm: out = RMS norm of s = x + resid, times w; s goes to resid_out (which may be resid).  out of
     torch.float8_e4m3fn takes e4m3 codes and scales their f32 scale per row; rstd (f32) is kept for the backward."""
-    shape, dev = _two_d("x", x), x.get_device()
+    xp, ldx, shape, dev = _first("x", x)
     rows, h = shape
-    xp, ldx = _mat("x", x, shape, dev)
-    op, ldo = _mat("out", out, shape, dev)
-    rp = sp = None
+    op, ldo = _mat("out", out, shape, dev, out.dtype)
+    rp = sp = cp = tp = None
     rt = ldr = lds = 0
+    if scales is not None:
+        cp = _vec("scales", scales, rows, dev)
+    if rstd is not None:
+        tp = _vec("rstd", rstd, rows, dev)
     if resid is not None or resid_out is not None:
+        dt = (resid_out if resid is None else resid).dtype
         rt = _type(resid_out if resid is None else resid)
-        rp, ldr = _mat("resid", resid, shape, dev)
-        sp, lds = _mat("resid_out", resid_out, shape, dev, None if resid is None else resid.dtype)
+        rp, ldr = _mat("resid", resid, shape, dev, dt)
+        sp, lds = _mat("resid_out", resid_out, shape, dev, dt)
     check(lib().jh_op_rms_norm(_type(x), xp, ldx, rt, rp, ldr, sp, lds, rows, h, _vec("w", w, h, dev), eps, _type(out),
-                               op, ldo, _vec("scales", scales, rows, dev), _vec("rstd", rstd, rows, dev), stream))
+                               op, ldo, cp, tp, stream))
 
 
 def op_rms_norm_backward(dy, s, w, rstd, ds, dw=None, workspace=None, dres=None, stream=None):
     """jh_op_rms_norm_backward: ds (+ dres) and dw from dy, with s = resid_out (or x) and rstd of op_rms_norm; dw
     needs a workspace tensor of rms_norm_backward_workspace(rows, hidden) bytes."""
-    shape, dev = _two_d("dy", dy), dy.get_device()
+    yp, ldy, shape, dev = _first("dy", dy)
     rows, h = shape
-    (yp, ldy), (sp, lds), (dp, ldd) = _mat("dy", dy, shape, dev), _mat("s", s, shape, dev), _mat("ds", ds, shape, dev)
+    (sp, lds), (dp, ldd) = _mat("s", s, shape, dev, s.dtype), _mat("ds", ds, shape, dev, ds.dtype)
     rp, ldr = _mat("dres", dres, shape, dev, ds.dtype)
     wp, wb = _space(workspace, dev)
     check(lib().jh_op_rms_norm_backward(_type(dy), yp, ldy, _type(s), sp, lds, rows, h, _vec("w", w, h, dev),
@@ -461,9 +476,9 @@ def rms_norm_backward_workspace(rows, hidden) -> int:
 
 def op_quantize_rows(x, q, scales, stream=None):
     """jh_op_quantize_rows: e4m3 codes q (torch.float8_e4m3fn) of x's rows and their f32 scales."""
-    shape, dev = _two_d("x", x), x.get_device()
+    xp, ldx, shape, dev = _first("x", x)
     rows, n = shape
-    (xp, ldx), (qp, ldq) = _mat("x", x, shape, dev), _mat("q", q, shape, dev)
+    qp, ldq = _mat("q", q, shape, dev, q.dtype)
     if _type(q) != abi.E4M3:
         _invalid("q: needs torch.float8_e4m3fn")
     check(lib().jh_op_quantize_rows(_type(x), xp, ldx, rows, n, qp, ldq, _vec("scales", scales, rows, dev), stream))
@@ -472,31 +487,39 @@ def op_quantize_rows(x, q, scales, stream=None):
 def op_linear(x, w, out, bias=None, act="none", resid=None, x_scale=None, w_scale=None, pre=None, stream=None):
     """jh_op_linear: out = act(x w^T + bias) + resid; x and w of one type (bf16, f16, or float8_e4m3fn with x_scale and
     w_scale), out f32 or their type (bf16 for e4m3); resid may be out; pre keeps x w^T + bias for the backward."""
-    rows, k = _two_d("x", x)
-    n, dev, dt = w.shape[0], x.get_device(), x.dtype
+    xp, ldx, (rows, k), dev = _first("x", x)
+    n, dt, ot = w.shape[0], x.dtype, out.dtype
     shape = (rows, n)
-    xp, ldx = _mat("x", x, x.shape, dev)
-    op, ldo = _mat("out", out, shape, dev)
-    rp, ldr = (None, 0) if resid is None else _mat("resid", resid, shape, dev, out.dtype)
-    pp, ldp = (None, 0) if pre is None else _mat("pre", pre, shape, dev, dt)
-    check(lib().jh_op_linear(_type(x), xp, ldx, _vec("x_scale", x_scale, rows, dev), rows,
-                             _weight("w", w, (n, k), dev, dt), _vec("w_scale", w_scale, n, dev), n, k,
-                             _vec("bias", bias, n, dev), _act(act), rp, ldr, _type(out), op, ldo, pp, ldp, stream))
+    op, ldo = _mat("out", out, shape, dev, ot)
+    rp = pp = xs = ws = bp = None
+    ldr = ldp = 0
+    if resid is not None:
+        rp, ldr = _mat("resid", resid, shape, dev, ot)
+    if pre is not None:
+        pp, ldp = _mat("pre", pre, shape, dev, dt)
+    if x_scale is not None:
+        xs = _vec("x_scale", x_scale, rows, dev)
+    if w_scale is not None:
+        ws = _vec("w_scale", w_scale, n, dev)
+    if bias is not None:
+        bp = _vec("bias", bias, n, dev)
+    check(lib().jh_op_linear(_type(x), xp, ldx, xs, rows, _weight("w", w, (n, k), dev, dt), ws, n, k, bp, _act(act), rp,
+                             ldr, _type(out), op, ldo, pp, ldp, stream))
 
 
 def op_linear_backward(dy, x, w, workspace, act="none", pre=None, dx=None, dw=None, dbias=None, stream=None):
     """jh_op_linear_backward: whichever of dx, dw (f32 or x's type) and dbias (f32) are given, from dy and (act not
     "none") pre; workspace of linear_backward_workspace(rows, n, k, act) bytes."""
-    shape, dev, dt = _two_d("dy", dy), dy.get_device(), dy.dtype
+    yp, ldy, shape, dev = _first("dy", dy)
     rows, n = shape
-    k = w.shape[1]
-    yp, ldy = _mat("dy", dy, shape, dev)
+    k, dt = w.shape[1], dy.dtype
     (xp, ldx), (dp, ldd) = _mat("x", x, (rows, k), dev, dt), _mat("dx", dx, (rows, k), dev, dt)
     pp, ldp = _mat("pre", pre, shape, dev, dt)
     wp, wb = _space(workspace, dev)
     check(lib().jh_op_linear_backward(_type(dy), yp, ldy, xp, ldx, rows, _weight("w", w, (n, k), dev, dt), n, k,
                                       _act(act), pp, ldp, dp, ldd, _type(dy if dw is None else dw),
-                                      _weight("dw", dw, (n, k), dev), _vec("dbias", dbias, n, dev), wp, wb, stream))
+                                      _weight("dw", dw, (n, k), dev, dt if dw is None else dw.dtype),
+                                      _vec("dbias", dbias, n, dev), wp, wb, stream))
 
 
 def linear_backward_workspace(rows, n, k, act="none") -> int:
@@ -506,32 +529,36 @@ def linear_backward_workspace(rows, n, k, act="none") -> int:
 def op_gated_ffn(x, wi, out, act="gelu", x_scale=None, w_scale=None, gu=None, stream=None):
     """jh_op_gated_ffn: out = act(x Wg^T) * (x Wu^T), wi = [Wg; Wu]; types as op_linear (out of x's type, bf16 for
     e4m3); gu [rows, 2 inter] keeps both projections for the backward."""
-    rows, k = _two_d("x", x)
-    n, dev, dt, code = wi.shape[0], x.get_device(), x.dtype, _type(x)
+    xp, ldx, (rows, k), dev = _first("x", x)
+    n, dt, code = wi.shape[0], x.dtype, _type(x)
     if n % 2:
         _invalid("wi: needs an even number of rows")
     if _type(out) != (abi.BF16 if code == abi.E4M3 else code):
         _invalid("out: has x's type (bfloat16 for e4m3)")
-    xp, ldx = _mat("x", x, x.shape, dev)
-    op, ldo = _mat("out", out, (rows, n // 2), dev)
-    gp, ldg = (None, 0) if gu is None else _mat("gu", gu, (rows, n), dev, dt)
-    check(lib().jh_op_gated_ffn(code, xp, ldx, _vec("x_scale", x_scale, rows, dev), rows,
-                                _weight("wi", wi, (n, k), dev, dt), _vec("w_scale", w_scale, n, dev), n // 2, k,
-                                _act(act), op, ldo, gp, ldg, stream))
+    op, ldo = _mat("out", out, (rows, n // 2), dev, out.dtype)
+    gp = xs = ws = None
+    ldg = 0
+    if gu is not None:
+        gp, ldg = _mat("gu", gu, (rows, n), dev, dt)
+    if x_scale is not None:
+        xs = _vec("x_scale", x_scale, rows, dev)
+    if w_scale is not None:
+        ws = _vec("w_scale", w_scale, n, dev)
+    check(lib().jh_op_gated_ffn(code, xp, ldx, xs, rows, _weight("wi", wi, (n, k), dev, dt), ws, n // 2, k, _act(act), op,
+                                ldo, gp, ldg, stream))
 
 
 def op_gated_ffn_backward(dh, gu, x, wi, workspace, act="gelu", dx=None, dw=None, stream=None):
     """jh_op_gated_ffn_backward: dx and / or dw (of wi; f32 or x's type) from dh and gu; workspace of
     gated_ffn_backward_workspace(rows, inter, k) bytes."""
-    shape, dev, dt = _two_d("dh", dh), dh.get_device(), dh.dtype
-    rows, inter = shape
-    k, n = wi.shape[1], 2 * inter
-    (hp, ldh), (gp, ldg) = _mat("dh", dh, shape, dev), _mat("gu", gu, (rows, n), dev, dt)
+    hp, ldh, (rows, inter), dev = _first("dh", dh)
+    k, n, dt = wi.shape[1], 2 * inter, dh.dtype
+    gp, ldg = _mat("gu", gu, (rows, n), dev, dt)
     (xp, ldx), (dp, ldd) = _mat("x", x, (rows, k), dev, dt), _mat("dx", dx, (rows, k), dev, dt)
     wp, wb = _space(workspace, dev)
     check(lib().jh_op_gated_ffn_backward(_type(dh), hp, ldh, gp, ldg, xp, ldx, rows, _weight("wi", wi, (n, k), dev, dt),
                                          inter, k, _act(act), dp, ldd, _type(dh if dw is None else dw),
-                                         _weight("dw", dw, (n, k), dev), wp, wb, stream))
+                                         _weight("dw", dw, (n, k), dev, dt if dw is None else dw.dtype), wp, wb, stream))
 
 
 def gated_ffn_backward_workspace(rows, inter, k) -> int:
