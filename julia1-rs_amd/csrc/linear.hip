@@ -181,7 +181,9 @@ double cost(int kernel, const LinearArgs& a, long splits) {
         }
         case DEEP: {
             const double t = (double)(tiles_of(a, 128, 128) * splits);
-            return rounds(t, CUS) * (s * (0.35 + 0.19 * load(t)) + 3.0) + 1.0;
+            // transposing reads move half as much per instruction, and this kernel waits for LDS most
+            const double by_cols = a.layout == COLS_COLS ? 1.4 : a.layout == COLS_ROWS ? 1.15 : 1.0;
+            return rounds(t, CUS) * (s * (0.35 + 0.19 * load(t)) * by_cols + 3.0) + 1.0;
         }
         case PAIR: {
             const double t = (double)(tiles_of(a, 128, 128) * splits);
@@ -189,7 +191,7 @@ double cost(int kernel, const LinearArgs& a, long splits) {
         }
         default: {
             const double t = (double)(tiles_of(a, 256, 256) * splits);
-            return rounds(t, CUS) * (s * (1.0 + 0.35 * load(t)) + 6.0) + 1.0;
+            return rounds(t, CUS) * (s * (1.0 + 0.4 * load(t)) + 6.0) + 1.0;
         }
     }
 }
@@ -201,14 +203,16 @@ struct Choice {
 };
 
 // The cheapest kernel and, for gradients, number of parts of the contraction, whose FP32 sums
-// take `splits` outputs' worth of memory (at most 16, and 48 MiB) and one more kernel.
-constexpr long MAX_SPLITS = 16, SPLIT_BYTES = 48L << 20, MIN_STEPS = 4;
+// take `splits` outputs' worth of memory (at most 16; 48 MiB of rows' gradients, 192 MiB of
+// weights') and one more kernel.
+constexpr long MAX_SPLITS = 16, MIN_STEPS = 4;
+long split_bytes(const LinearArgs& a) { return (a.layout == COLS_COLS ? 192L : 48L) << 20; }
 Choice pick(const LinearArgs& a, bool gradient) {
     Choice best{PAIR, 1, 1e30};
     const double out = (double)a.q_rows * a.p_cols * 4;
     for (long splits = 1; splits <= (gradient ? MAX_SPLITS : 1); splits += splits < 4 ? 1 : splits < 8 ? 2 : 4) {
-        if (splits > 1 && (steps_of(a) < splits * MIN_STEPS || out * splits > SPLIT_BYTES)) break;
-        const double sum = splits > 1 ? 2.5 + (splits + 1) * out / 4.5e6 : 0.0;
+        if (splits > 1 && (steps_of(a) < splits * MIN_STEPS || out * splits > split_bytes(a))) break;
+        const double sum = splits > 1 ? 2.5 + (2 * splits + 0.5) * out / 4.5e6 : 0.0;  // written and read
         for (int kernel = 0; kernel < KERNELS; ++kernel) {
             if (kernel == WIDE && a.type == JH_E4M3 && a.out_f32) continue;  // has no bf16 fragments of e4m3
             const double c = cost(kernel, a, splits) + sum;

@@ -358,11 +358,14 @@ __device__ inline void finish_gated8(const LinearArgs& a, float (&g)[8], float (
 }
 
 // Epilogue of a wave's block of 64 P rows and 16 NJ output rows, the first of them t0; col0
-// is its first output column.  Residuals are loaded two row blocks at a time, into the
+// is its first output column.  HALF: after that many blocks of 16 rows (and, where P is by
+// columns, after 32 columns) the rest lies 128 rows (columns) beyond the block's first.  Residuals are loaded two row blocks at a time, into the
 // registers that the fragments no longer need.
-template <class T, int LAYOUT, int EPI, int NJ>
+template <class T, int LAYOUT, int EPI, int NJ, int HALF = NJ>
 __device__ inline void finish(const LinearArgs& a, f32x4 (&acc)[4][NJ], int t0, int col0, int lane, int split) {
-    const int g = lane >> 4, c0 = col0 + g * (EPI == EPI_GATED ? 8 : 16);
+    const int g = lane >> 4;
+    const int c0 = col0 + (HALF < NJ && LAYOUT != ROWS_ROWS ? (g & 1) * 16 + (g >> 1) * 128 : g * (EPI == EPI_GATED ? 8 : 16));
+    auto row_of_block = [&](int j) { return t0 + (j < HALF ? j * 16 : 128 + (j - HALF) * 16) + (lane & 15); };
     ColumnTerms<T> col[2];
     constexpr int AHEAD = NJ > 2 ? 2 : 1;
     Resid8 resid[AHEAD][2];
@@ -378,11 +381,11 @@ __device__ inline void finish(const LinearArgs& a, f32x4 (&acc)[4][NJ], int t0, 
             for (int i = 0; i < AHEAD; ++i)
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
-                    if (j + i < NJ) resid[i][h].load(a, t0 + (j + i) * 16 + (lane & 15), c0 + 8 * h);
+                    if (j + i < NJ) resid[i][h].load(a, row_of_block(j + i), c0 + 8 * h);
         }
         f32x4 c[4] = {acc[0][j], acc[1][j], acc[2][j], acc[3][j]};
         if constexpr (LAYOUT != ROWS_ROWS) transpose_groups(c);
-        const long t = t0 + j * 16 + (lane & 15);
+        const long t = row_of_block(j);
         const float qs = T::bytes == 1 && a.q_scale ? a.q_scale[min(t, (long)a.q_rows - 1)] : 1.0f;
         if (t < a.q_rows) {
             if constexpr (EPI == EPI_GATED) {

@@ -18,8 +18,12 @@
 // The two waves of a SIMD (w and w + 4) run one half phase apart, waves 4-7 having met one
 // barrier more: while one multiplies, the other reads and issues.
 //
-// LDS holds two K steps of four 16 KB parts: Pa and Pb the first and second 32 rows of every
-// wave column, Qa and Qb the first and second 64 rows of the two wave rows.  A part read in
+// LDS holds two K steps of four 16 KB parts: Qa and Qb are the tile's first and last 128 Q
+// rows, 64 of each for a wave; Pa and Pb the first and second 32 P rows of every wave column
+// where k is contiguous (whatever rows, a lane ends with 16 consecutive output columns), the
+// tile's first and last 128 columns where k is the row index (there, a part read in two runs of
+// 128 bytes or four of 64 per row instead of one of 256 cost dW of 29367 x 3464 x 1504
+// 426 us against 3XX).  A part read in
 // one phase is refilled in the next: every wave has waited for its own reads (lgkmcnt) before
 // the barrier that the refilling waves have passed.  A part is read seven phases after its
 // issue, and one phase after every wave has waited for its own share of it: a wave issues two
@@ -55,8 +59,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     // halves of an operand: the second half lies p_half (q_half) bytes further.
     const uint8_t* const pb = (const uint8_t*)a.p + (P_COLS ? (long)p0 : (long)p0 * a.ldp) * ES;
     const uint8_t* const qb = (const uint8_t*)a.q + (Q_COLS ? (long)q0 : (long)q0 * a.ldq) * ES;
-    const long p_half = P_COLS ? 32 * ES : (EPI == EPI_GATED ? (long)a.p_cols : 8L) * a.ldp * ES;
-    const long q_half = (Q_COLS ? 64L : 64 * a.ldq) * ES;
+    const long p_half = P_COLS ? 128 * ES : (EPI == EPI_GATED ? (long)a.p_cols : 8L) * a.ldp * ES;
+    const long q_half = (Q_COLS ? 128L : 128 * a.ldq) * ES;
     const int p_rows = EPI == EPI_GATED ? 2 * a.p_cols - p0 : a.p_cols - p0;
     const long p_bytes = ((long)(p_rows - 1) * a.ldp + a.k) * ES, q_bytes = ((long)(a.q_rows - q0 - 1) * a.ldq + a.k) * ES;
     i32x4 rp[2], rq[2];
@@ -75,10 +79,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         const int k = (wave * 2 + j) * 4 + (lane >> 4), q = (lane & 15) ^ col_swz<128>(k);  // row and chunk of a part by columns
         const uint32_t rk = ((lane & 7) ^ row_swz(r)) * 16;
         tail[j] = __builtin_amdgcn_ballot_w64((steps - 1) * STEP_BYTES + rk < kbytes);
-        poff[j] = P_COLS ? (uint32_t)((k * a.ldp + (q >> 2) * 64 + (q & 3) * 8) * ES)
+        poff[j] = P_COLS ? (uint32_t)((k * a.ldp + q * 8) * ES)
                          : (uint32_t)(p_row<EPI>((r >> 5) * 64 + (r & 31), a.p_cols) * a.ldp * ES + rk);
-        qoff[j] = Q_COLS ? (uint32_t)((k * a.ldq + (q >> 3) * 128 + (q & 7) * 8) * ES)
-                         : (uint32_t)(((r >> 6) * 128 + (r & 63)) * a.ldq * ES + rk);
+        qoff[j] = Q_COLS ? (uint32_t)((k * a.ldq + q * 8) * ES) : (uint32_t)(r * a.ldq * ES + rk);
     }
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)&smem[wave * 2048]);
     const int split = blockIdx.y, kt0 = min(split * a.split_steps, steps), kt1 = min(kt0 + a.split_steps, steps);
@@ -171,9 +174,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     // No load may still be on its way into LDS when the workgroup ends.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
-    const int col0 = p0 + wp * (EPI == EPI_GATED ? 32 : 64);
+    const int col0 = p0 + wp * (EPI == EPI_GATED || P_COLS ? 32 : 64);
     const int l = (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0));  // `lane`, not kept over the loop
-    finish<T, LAYOUT, EPI, 8>(a, acc, q0 + wq * 128, col0, l, split);
+    // The second half of the wave's Q rows lies 128 rows on; of its P columns (by columns) too.
+    finish<T, LAYOUT, EPI, 8, 4>(a, acc, q0 + wq * 64, col0, l, split);
 }
 
 template <class T, int LAYOUT, int EPI>
