@@ -116,10 +116,20 @@ __global__ __launch_bounds__(THREADS) void split_sum_kernel(const float* partial
     if (r >= rows) return;
     const long plane = (long)rows * cols;
     const float* p = partial + r * cols + c;
-    f32x4 lo = *(const f32x4*)p, hi = *(const f32x4*)(p + 4);
-    for (int s = 1; s < splits; ++s) {
-        lo += *(const f32x4*)(p + s * plane);
-        hi += *(const f32x4*)(p + s * plane + 4);
+    f32x4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
+    for (int s0 = 0; s0 < splits; s0 += 4) {  // four planes in flight; those past the last are read again, not added
+        f32x4 v[4][2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) v[i][h] = *(const f32x4*)(p + min(s0 + i, splits - 1) * plane + 4 * h);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (s0 + i < splits) {
+                lo += v[i][0];
+                hi += v[i][1];
+            }
+        }
     }
     if (out_f32) {
         float* o = (float*)out + r * ldo + c;

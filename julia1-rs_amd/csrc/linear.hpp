@@ -359,64 +359,83 @@ __device__ inline void finish_gated8(const LinearArgs& a, float (&g)[8], float (
 
 // Epilogue of a wave's block of 64 P rows and 16 NJ output rows, the first of them t0; col0
 // is its first output column.  HALF: after that many blocks of 16 rows (and, where P is by
-// columns, after 32 columns) the rest lies 128 rows (columns) beyond the block's first.  Residuals are loaded two row blocks at a time, into the
-// registers that the fragments no longer need.
-template <class T, int LAYOUT, int EPI, int NJ, int HALF = NJ>
-__device__ inline void finish(const LinearArgs& a, f32x4 (&acc)[4][NJ], int t0, int col0, int lane, int split) {
-    const int g = lane >> 4;
-    const int c0 = col0 + (HALF < NJ && LAYOUT != ROWS_ROWS ? (g & 1) * 16 + (g >> 1) * 128 : g * (EPI == EPI_GATED ? 8 : 16));
-    auto row_of_block = [&](int j) { return t0 + (j < HALF ? j * 16 : 128 + (j - HALF) * 16) + (lane & 15); };
+// columns, after 32 columns) the rest lies 128 rows (columns) beyond the block's first.
+// EARLY: what the epilogue reads is loaded by start(), under the multiplications; without it,
+// column terms by finish() and residuals two row blocks ahead of their use, into the registers
+// that the fragments no longer need.
+template <class T, int LAYOUT, int EPI, int NJ, int HALF, bool EARLY>
+struct Epilogue {
+    static constexpr int AHEAD = EARLY ? NJ : NJ > 2 ? 2 : 1;
+    const LinearArgs& a;
+    int t0, c0, lane;
     ColumnTerms<T> col[2];
-    constexpr int AHEAD = NJ > 2 ? 2 : 1;
     Resid8 resid[AHEAD][2];
-    if (!a.partial) {
+
+    __device__ Epilogue(const LinearArgs& args, int row0, int col0, int lane_id) : a(args), t0(row0), lane(lane_id) {
+        const int g = lane >> 4;
+        c0 = col0 + (HALF < NJ && LAYOUT != ROWS_ROWS ? (g & 1) * 16 + (g >> 1) * 128 : g * (EPI == EPI_GATED ? 8 : 16));
+    }
+    __device__ int row(int j) const { return t0 + (j < HALF ? j * 16 : 128 + (j - HALF) * 16) + (lane & 15); }
+    __device__ void load_columns() {
+        if (a.partial) return;
         col[0].load(a, c0, a.p_scale);
         if constexpr (EPI == EPI_GATED) col[1].load(a, c0, a.p_scale ? a.p_scale + a.p_cols : nullptr);
         else col[1].load(a, c0 + 8, a.p_scale);
     }
+    __device__ void load_residuals(int j) {  // of row blocks j .. j + AHEAD - 1
+        if (EPI == EPI_GATED || !a.resid) return;
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-        if (EPI == EPI_LINEAR && a.resid && j % AHEAD == 0) {
+        for (int i = 0; i < AHEAD; ++i)
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    if (j + i < NJ) resid[i][h].load(a, row_of_block(j + i), c0 + 8 * h);
+            for (int h = 0; h < 2; ++h)
+                if (j + i < NJ) resid[i][h].load(a, row(j + i), c0 + 8 * h);
+    }
+    __device__ void start() {
+        if constexpr (EARLY) {
+            load_columns();
+            load_residuals(0);
         }
-        f32x4 c[4] = {acc[0][j], acc[1][j], acc[2][j], acc[3][j]};
-        if constexpr (LAYOUT != ROWS_ROWS) transpose_groups(c);
-        const long t = row_of_block(j);
-        const float qs = T::bytes == 1 && a.q_scale ? a.q_scale[min(t, (long)a.q_rows - 1)] : 1.0f;
-        if (t < a.q_rows) {
-            if constexpr (EPI == EPI_GATED) {
-                float ga[8], up[8];
+    }
+    __device__ void finish(f32x4 (&acc)[4][NJ], int split) {
+        if constexpr (!EARLY) load_columns();
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    ga[e] = c[e >> 2][e & 3];
-                    up[e] = c[2 + (e >> 2)][e & 3];
-                }
-                if (c0 < a.p_cols) finish_gated8<T>(a, ga, up, t, c0, qs, col[0], col[1]);
-            } else {
+        for (int j = 0; j < NJ; ++j) {
+            if (!EARLY && j % AHEAD == 0) load_residuals(j);
+            f32x4 c[4] = {acc[0][j], acc[1][j], acc[2][j], acc[3][j]};
+            if constexpr (LAYOUT != ROWS_ROWS) transpose_groups(c);
+            const long t = row(j);
+            const float qs = T::bytes == 1 && a.q_scale ? a.q_scale[min(t, (long)a.q_rows - 1)] : 1.0f;
+            if (t < a.q_rows) {
+                if constexpr (EPI == EPI_GATED) {
+                    float ga[8], up[8];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int ch = c0 + 8 * h;
-                    if (ch >= a.p_cols) continue;
-                    if (a.partial) {
-                        float* o = a.partial + ((long)split * a.q_rows + t) * a.p_cols + ch;
-                        *(f32x4*)o = c[2 * h];
-                        *(f32x4*)(o + 4) = c[2 * h + 1];
-                    } else {
-                        float z[8];
+                    for (int e = 0; e < 8; ++e) {
+                        ga[e] = c[e >> 2][e & 3];
+                        up[e] = c[2 + (e >> 2)][e & 3];
+                    }
+                    if (c0 < a.p_cols) finish_gated8<T>(a, ga, up, t, c0, qs, col[0], col[1]);
+                } else {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) z[e] = c[2 * h + (e >> 2)][e & 3];
-                        finish8<T>(a, z, t, ch, qs, col[h], resid[j % AHEAD][h]);
+                    for (int h = 0; h < 2; ++h) {
+                        const int ch = c0 + 8 * h;
+                        if (ch >= a.p_cols) continue;
+                        if (a.partial) {
+                            float* o = a.partial + ((long)split * a.q_rows + t) * a.p_cols + ch;
+                            *(f32x4*)o = c[2 * h];
+                            *(f32x4*)(o + 4) = c[2 * h + 1];
+                        } else {
+                            float z[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) z[e] = c[2 * h + (e >> 2)][e & 3];
+                            finish8<T>(a, z, t, ch, qs, col[h], resid[j % AHEAD][h]);
+                        }
                     }
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
-        __builtin_amdgcn_sched_barrier(0);
     }
-}
+};
 
 // Tile order: workgroup b runs on XCD b % 8, so each XCD gets a contiguous band of tiles,
 // swept GROUP row blocks at a time for every column block, which keeps the operands that

@@ -96,6 +96,10 @@ __global__ __launch_bounds__(64 * WP * WQ * KG) __attribute__((amdgpu_waves_per_
         }
     };
 
+    // Where registers are free for it, the epilogue's operands come in before the loop.
+    Epilogue<T, LAYOUT, EPI, NJ, NJ, KG == 1 && NJ <= 2> epilogue(a, q0 + wq * 16 * NJ, p0 + wp * (EPI == EPI_GATED ? 32 : 64),
+                                                                 lane);
+    epilogue.start();
     f32x4 acc[4][NJ];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -173,7 +177,7 @@ __global__ __launch_bounds__(64 * WP * WQ * KG) __attribute__((amdgpu_waves_per_
             for (int i = 0; i < 4 * NJ; ++i) acc[i / NJ][i % NJ] += sums[g * GROUP + i * 64];
     }
 
-    finish<T, LAYOUT, EPI, NJ>(a, acc, q0 + wq * 16 * NJ, p0 + wp * (EPI == EPI_GATED ? 32 : 64), lane, split);
+    epilogue.finish(acc, split);
 }
 
 template <class T, int LAYOUT, int EPI, int WP, int WQ, int NJ, int KG, int NST>

@@ -177,7 +177,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int col0 = p0 + wp * (EPI == EPI_GATED || P_COLS ? 32 : 64);
     const int l = (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0));  // `lane`, not kept over the loop
     // The second half of the wave's Q rows lies 128 rows on; of its P columns (by columns) too.
-    finish<T, LAYOUT, EPI, 8, 4>(a, acc, q0 + wq * 64, col0, l, split);
+    Epilogue<T, LAYOUT, EPI, 8, 4, false>(a, q0 + wq * 64, col0, l).finish(acc, split);
 }
 
 template <class T, int LAYOUT, int EPI>
