@@ -21,9 +21,9 @@
 // LDS holds two K steps of four 16 KB parts: Qa and Qb are the tile's first and last 128 Q
 // rows, 64 of each for a wave; Pa and Pb the first and second 32 P rows of every wave column
 // where k is contiguous (whatever rows, a lane ends with 16 consecutive output columns), the
-// tile's first and last 128 columns where k is the row index (there, a part read in two runs of
-// 128 bytes or four of 64 per row instead of one of 256 cost dW of 29367 x 3464 x 1504
-// 426 us against 3XX).  A part read in
+// tile's first and last 128 columns where k is the row index (one run of 256 bytes per row;
+// the weight gradient of 29367 x 3464 x 1504 took 403 us so, 426 in two runs of 128 and four
+// of 64).  A part read in
 // one phase is refilled in the next: every wave has waited for its own reads (lgkmcnt) before
 // the barrier that the refilling waves have passed.  A part is read seven phases after its
 // issue, and one phase after every wave has waited for its own share of it: a wave issues two

@@ -373,14 +373,25 @@ def _type(t):
 # These run before every launch of a few microseconds, so they ask a tensor for no more than they need.
 
 def _first(name, t):
-    """(address, row stride, shape, device) of an operator's first operand, a 2-D tensor."""
+    """(address, row stride, shape, device) of an operator's first operand, a 2-D tensor on the current device (where
+    the kernels are launched)."""
     shape = t.shape
     if len(shape) != 2:
         _invalid(f"{name}: needs a matrix")
     ld, one = t.stride()
     if one != 1 and shape[1] > 1:
         _invalid(f"{name}: needs contiguous rows")
-    return t.data_ptr(), ld, shape, t.get_device()
+    dev = t.get_device()
+    if dev < 0 or dev != _current_device():
+        _invalid(f"{name}: on {t.device}, which is not the current device")
+    return t.data_ptr(), ld, shape, dev
+
+
+def _current_device():
+    global _current_device
+    import torch
+    _current_device = torch.cuda.current_device
+    return _current_device()
 
 
 def _mat(name, t, shape, dev, dtype):

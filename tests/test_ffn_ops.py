@@ -122,9 +122,23 @@ def test_gated_backward_refusals(change):
     assert refused(hip.lib().jh_op_gated_ffn_backward, GATED_B, **change)
 
 
-def test_column_ranges_of_one_buffer_do_not_overlap():
-    """Two column ranges of one buffer may be input and output; ranges that share a column may not.  No rows are
-    computed: the refusals of bad layouts come before, so an accepted call is one that only a missing device ends."""
+def test_host_tensors_are_refused():
+    """The Python calls take tensors of the current device alone: an address of host memory would fault there."""
+    torch = pytest.importorskip("torch")
+    x, w, out = torch.zeros(4, 64), torch.zeros(32, 64), torch.zeros(4, 32)
+    for call in (lambda: hip.op_linear(x, w, out), lambda: hip.op_gated_ffn(x, w, out[:, :16]),
+                 lambda: hip.op_rms_norm(x, torch.ones(64), 1e-6, x.bfloat16()),
+                 lambda: hip.op_quantize_rows(x, torch.zeros(4, 64, dtype=torch.float8_e4m3fn), torch.zeros(4)),
+                 lambda: hip.op_rms_norm_backward(x, x, torch.ones(64), torch.ones(4), x.clone()),
+                 lambda: hip.op_linear_backward(out, x, w, None, dx=x), lambda: hip.op_gated_ffn_backward(
+                     out[:, :16], out, x, w, None, dx=x)):
+        with pytest.raises(hip.HipError) as e:
+            call()
+        assert e.value.code == abi.JH_ERR_INVALID and "current device" in str(e.value)
+
+
+def test_column_ranges_of_one_buffer_that_share_a_column():
+    """Ranges of one buffer's columns that share one are refused, also where a range wraps onto the next row."""
     base = dict(LINEAR, resid=None, pre=None, bias=None, ot=abi.BF16, x=at(0), ldx=256, ldo=256, n=32)
     refused(hip.lib().jh_op_linear, base, out=at(0) + 2 * 48)      # columns 48 .. 79 over x's 0 .. 63
     refused(hip.lib().jh_op_linear, base, out=at(0) + 2 * 240)     # 240 .. 271 wrap onto the next row's first

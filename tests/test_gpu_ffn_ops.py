@@ -306,6 +306,31 @@ def test_linear(rows, n, k, t, out_t):
                 t != E4M3 and i % 4 < 2, seed=100 + i)
 
 
+# one size for each kernel that larger products run on: 128 x 128 tiles one to a CU and two to a CU, 256 x 256 tiles,
+# those for whole rounds of the CUs with the rest on smaller ones, and 64 x 64 tiles whose waves share a long contraction
+KERNELS = [(1000, 4000, 520), (1500, 4000, 520), (3900, 4000, 520), (4700, 4000, 520), (129, 264, 4104)]
+
+
+@pytest.mark.parametrize("rows,n,k", KERNELS)
+@pytest.mark.parametrize("t,out_t", [(BF16, BF16), (F16, F32), (E4M3, BF16), (E4M3, F32)])
+def test_linear_kernels(rows, n, k, t, out_t):
+    linear_case(rows, n, k, t, out_t, "silu", True, True, t != E4M3, seed=rows)
+
+
+@pytest.mark.parametrize("rows,n,k", KERNELS)
+@pytest.mark.parametrize("t", [BF16, F16, E4M3])
+def test_gated_ffn_kernels(rows, n, k, t):
+    test_gated_ffn(rows, n // 16 * 8, k, t)
+
+
+# the same for both gradients (dx: rows x k over n; dw: n x k over rows), and contractions that are cut into parts
+@pytest.mark.parametrize("rows,n,k", [(1500, 520, 4000), (3900, 520, 4000), (4700, 520, 4000), (520, 1504, 4000),
+                                      (520, 3904, 4000), (520, 4704, 4000), (9000, 1032, 776), (264, 6008, 264)])
+@pytest.mark.parametrize("t,grad_t", [(BF16, BF16), (F16, F32)])
+def test_linear_backward_kernels(rows, n, k, t, grad_t):
+    test_linear_backward(rows, n, k, t, grad_t, "gelu")
+
+
 @pytest.mark.parametrize("act", ["none", "relu", "gelu", "gelu_tanh", "silu"])
 @pytest.mark.parametrize("rows", [3, 200])
 def test_linear_activations(act, rows):
@@ -609,3 +634,101 @@ def test_block_on_another_stream_and_in_a_graph():
         assert all(torch.equal(x, y) for x, y in zip(other.outputs(), want2))
         Block(64, 128, 72, F16, seed=7).step()
         torch.cuda.synchronize()
+
+
+def test_blocks_on_two_streams_at_once():
+    """Two blocks with workspaces of their own, on two streams without order between them."""
+    a, b = Block(700, 512, 520, BF16, seed=8), Block(700, 512, 520, BF16, seed=9)
+    a.step()
+    b.step()
+    torch.cuda.synchronize()
+    want = [t.clone() for t in a.outputs() + b.outputs()]
+    for t in a.outputs() + b.outputs():
+        t.zero_()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for blk, st in zip((a, b), streams):
+            with torch.cuda.stream(st):
+                blk.step(stream=st.cuda_stream)
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(a.outputs() + b.outputs(), want))
+
+
+# ---------------------------------------------------------------- far offsets
+
+def roomy(gib):
+    if torch.cuda.mem_get_info()[0] < gib << 30:
+        pytest.skip(f"needs {gib} GiB of free device memory")
+
+
+def some(rows):
+    """Row indices on both sides of 2^31 elements, the first and the last."""
+    return torch.tensor([0, 1, rows // 2, rows - 4000, rows - 2, rows - 1], device="cuda")
+
+
+def test_rows_past_2_31_elements_norms():
+    roomy(40)
+    rows, h = 140000, 16384
+    g = gen(11)
+    x = torch.empty(rows, h, device="cuda", dtype=BF16)
+    for i in range(0, rows, 20000):
+        x[i:i + 20000] = randn(g, 20000, h)[: rows - i]
+    w, out, q, scales = 1 + randn(g, h, std=0.2), torch.empty_like(x), torch.empty(rows, h, device="cuda", dtype=E4M3), \
+        torch.empty(rows, device="cuda")
+    rstd = torch.empty(rows, device="cuda")
+    hip.op_rms_norm(x, w, EPS, out, rstd=rstd)
+    hip.op_quantize_rows(x, q, scales)
+    torch.cuda.synchronize()
+    i = some(rows)
+    v = x[i].double()
+    y = v / torch.sqrt((v * v).mean(dim=1, keepdim=True) + EPS) * w.double()
+    close(out[i], y, y.abs() * (half(BF16) + (h + 32) * 2.0**-24), "out")
+    assert torch.equal(q[i].double(), nearest_e4m3(v * 448 / v.abs().amax(dim=1, keepdim=True)))
+    hip.op_rms_norm_backward(x, x, w, rstd, out)
+    torch.cuda.synchronize()
+    r = rstd[i].double()[:, None]
+    n, gy = v * r, v * w.double()
+    want = r * (gy - n * (gy * n).mean(dim=1, keepdim=True))
+    size = (gy * n).abs().mean(dim=1, keepdim=True)
+    close(out[i], want, r * (gy.abs() * 8 + n.abs() * size * (h + 16)) * 2.0**-24 + want.abs() * half(BF16), "ds")
+
+
+def test_rows_past_2_31_elements_products():
+    roomy(60)
+    rows, n, k = 70000, 32768, 64
+    g = gen(12)
+    x, w = randn(g, rows, k).to(BF16), randn(g, n, k, std=0.125).to(BF16)
+    out, pre = torch.empty(rows, n, device="cuda", dtype=BF16), torch.empty(rows, n, device="cuda", dtype=BF16)
+    hip.op_linear(x, w, out, act="relu", pre=pre)
+    torch.cuda.synchronize()
+    i = some(rows)
+    z = x[i].double() @ w.double().t()
+    tol = z.abs() * half(BF16) + (x[i].double().abs() @ w.double().abs().t()) * (k + 4) * 2.0**-23
+    close(pre[i], z, tol, "pre")
+    close(out[i], z.clamp_min(0), tol, "out")
+    # gradients: dy = out, a pre-activation that the relu passes on every other column
+    dx, dw = torch.empty_like(x), torch.empty(n, k, device="cuda")
+    ws = torch.empty(hip.linear_backward_workspace(rows, n, k, "relu"), dtype=torch.uint8, device="cuda")
+    hip.op_linear_backward(out, x, w, ws, act="relu", pre=pre, dx=dx, dw=dw)
+    torch.cuda.synchronize()
+    dz = out[i].double() * (pre[i] > 0)
+    want = dz @ w.double()
+    close(dx[i], want, want.abs() * half(BF16) + (dz.abs() @ w.double().abs()) * (n + 4) * 2.0**-23, "dx")
+    c = torch.tensor([0, 5, n // 2, n - 1], device="cuda")
+    dz = out[:, c].double() * (pre[:, c] > 0)
+    want = dz.t() @ x.double()
+    close(dw[c], want, (dz.abs().t() @ x.double().abs()) * (rows + 32) * 2.0**-23 + want.abs() * half(F32), "dw")
+    del out, pre, ws
+    inter = n // 2
+    h, gu = torch.empty(rows, inter, device="cuda", dtype=BF16), torch.empty(rows, n, device="cuda", dtype=BF16)
+    hip.op_gated_ffn(x, w, h, act="relu", gu=gu)
+    torch.cuda.synchronize()
+    close(gu[i], z, tol, "gu")
+    ws = torch.empty(hip.gated_ffn_backward_workspace(rows, inter, k), dtype=torch.uint8, device="cuda")
+    hip.op_gated_ffn_backward(h, gu, x, w, ws, act="relu", dx=dx)
+    torch.cuda.synchronize()
+    a, u, d = gu[i, :inter].double().clamp_min(0), gu[i, inter:].double(), h[i].double()
+    dz = torch.cat([d * u * (gu[i, :inter] > 0), d * a], dim=1)
+    want = dz @ w.double()
+    close(dx[i], want, want.abs() * half(BF16) + (dz.abs() @ w.double().abs()) * (half(BF16) * 1.01 + (n + 4) * 2.0**-23), "dx")
