@@ -293,14 +293,16 @@ struct ColumnTerms {
     }
 };
 
-// The residual of eight columns of one row, raw.
+// The residual of eight columns of one row, raw (e4m3 operands with FP32 outputs are E4m3Wide).
+template <class T>
 struct Resid8 {
-    u32x4 v[2];
+    static constexpr bool HALF_ONLY = __is_same(T, E4m3);
+    u32x4 v[HALF_ONLY ? 1 : 2];
     __device__ void load(const LinearArgs& a, long t, int c0) {
         const long at = min(t, (long)a.q_rows - 1) * a.ldr + min(c0, a.p_cols - 8);
-        if (a.out_f32) {
+        if (!HALF_ONLY && a.out_f32) {
             v[0] = *(const u32x4*)((const float*)a.resid + at);
-            v[1] = *(const u32x4*)((const float*)a.resid + at + 4);
+            v[HALF_ONLY ? 0 : 1] = *(const u32x4*)((const float*)a.resid + at + 4);
         } else {
             v[0] = *(const u32x4*)((const uint16_t*)a.resid + at);
         }
@@ -310,16 +312,16 @@ struct Resid8 {
 // Eight columns of one output row from their sums z: c0 .. c0+7.
 template <class T>
 __device__ inline void finish8(const LinearArgs& a, float (&z)[8], long t, int c0, float qs, const ColumnTerms<T>& col,
-                               const Resid8& resid) {
+                               const Resid8<T>& resid) {
     col.apply(a, z, qs);
     if constexpr (T::bytes == 2)
         if (a.pre) store16<T>((uint16_t*)a.pre + t * a.ldpre + c0, z);
     activate(z, a.act);
-    if (a.out_f32) {
+    if (!Resid8<T>::HALF_ONLY && a.out_f32) {
         if (a.resid) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const uint32_t r = resid.v[e >> 2][e & 3];
+                const uint32_t r = resid.v[Resid8<T>::HALF_ONLY ? 0 : e >> 2][e & 3];
                 z[e] += __builtin_bit_cast(float, r);
             }
         }
@@ -361,15 +363,16 @@ __device__ inline void finish_gated8(const LinearArgs& a, float (&g)[8], float (
 // is its first output column.  HALF: after that many blocks of 16 rows (and, where P is by
 // columns, after 32 columns) the rest lies 128 rows (columns) beyond the block's first.
 // EARLY: what the epilogue reads is loaded by start(), under the multiplications; without it,
-// column terms by finish() and residuals two row blocks ahead of their use, into the registers
+// column terms by finish() and residuals four row blocks at a time, into the registers
 // that the fragments no longer need.
 template <class T, int LAYOUT, int EPI, int NJ, int HALF, bool EARLY>
 struct Epilogue {
-    static constexpr int AHEAD = EARLY ? NJ : NJ > 2 ? 2 : 1;
+    static constexpr int AHEAD = EARLY || NJ < 4 ? NJ : 4;
     const LinearArgs& a;
     int t0, c0, lane;
     ColumnTerms<T> col[2];
-    Resid8 resid[AHEAD][2];
+    Resid8<T> resid[AHEAD][2];
+    float scale[NJ];  // of e4m3 rows
 
     __device__ Epilogue(const LinearArgs& args, int row0, int col0, int lane_id) : a(args), t0(row0), lane(lane_id) {
         const int g = lane >> 4;
@@ -381,6 +384,10 @@ struct Epilogue {
         col[0].load(a, c0, a.p_scale);
         if constexpr (EPI == EPI_GATED) col[1].load(a, c0, a.p_scale ? a.p_scale + a.p_cols : nullptr);
         else col[1].load(a, c0 + 8, a.p_scale);
+        if constexpr (T::bytes == 1) {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) scale[j] = a.q_scale ? a.q_scale[min(row(j), a.q_rows - 1)] : 1.0f;
+        }
     }
     __device__ void load_residuals(int j) {  // of row blocks j .. j + AHEAD - 1
         if (EPI == EPI_GATED || !a.resid) return;
@@ -404,7 +411,7 @@ struct Epilogue {
             f32x4 c[4] = {acc[0][j], acc[1][j], acc[2][j], acc[3][j]};
             if constexpr (LAYOUT != ROWS_ROWS) transpose_groups(c);
             const long t = row(j);
-            const float qs = T::bytes == 1 && a.q_scale ? a.q_scale[min(t, (long)a.q_rows - 1)] : 1.0f;
+            const float qs = T::bytes == 1 ? scale[j] : 1.0f;
             if (t < a.q_rows) {
                 if constexpr (EPI == EPI_GATED) {
                     float ga[8], up[8];

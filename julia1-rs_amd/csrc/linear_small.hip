@@ -65,7 +65,7 @@ __global__ __launch_bounds__(64 * NW) void linear_small_kernel(LinearArgs a) {
     if (half > 1 || row >= a.q_rows || c0 >= a.p_cols) return;
     const float qs = ES == 1 && a.q_scale ? a.q_scale[row] : 1.0f;
     ColumnTerms<T> col[PT];
-    Resid8 resid;
+    Resid8<T> resid;
 #pragma unroll
     for (int i = 0; i < PT; ++i) col[i].load(a, c0, a.p_scale ? a.p_scale + (long)i * a.p_cols : nullptr);
     if (a.resid) resid.load(a, row, c0);

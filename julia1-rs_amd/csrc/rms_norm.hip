@@ -413,6 +413,7 @@ __global__ __launch_bounds__(SUM_THREADS) void column_sum_kernel(const float* in
     __syncthreads();
     if (threadIdx.x < 64 && blockIdx.x * 64 + threadIdx.x < cols) {
         float t = 0.0f;
+#pragma unroll
         for (int g = 0; g < SUM_GROUPS; ++g) t += part[g][threadIdx.x];
         out[blockIdx.x * 64 + threadIdx.x] = t;
     }
