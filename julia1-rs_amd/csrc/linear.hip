@@ -375,7 +375,8 @@ void check_act(const char* op, int act) {
 
 }  // namespace
 
-void linear_forward(const LinearArgs& a, size_t rows, size_t n, size_t k, int out_type, hipStream_t s) {
+void linear_forward(const LinearArgs& args, size_t rows, size_t n, size_t k, int out_type, hipStream_t s) {
+    LinearArgs a = args;
     const char* op = a.gated ? "gated_ffn" : "linear";
     check_sizes(op, a.type, rows, n, k);
     check_act(op, a.act);
@@ -387,6 +388,10 @@ void linear_forward(const LinearArgs& a, size_t rows, size_t n, size_t k, int ou
     if (a.type == JH_E4M3 && a.pre) refuse(op, "pre-activations are kept for 16-bit operands");
     const size_t w_rows = a.gated ? 2 * n : n;
     if (rows == 0) return;
+    a.ldq = row_stride(a.ldq, rows, k);
+    a.ldo = row_stride(a.ldo, rows, n);
+    a.ldr = row_stride(a.ldr, rows, n);
+    a.ldpre = row_stride(a.ldpre, rows, w_rows);
     check_matrix(op, "x", a.q, a.ldq, rows, k, a.type);
     check_matrix(op, "w", a.p, a.ldp, w_rows, k, a.type);
     check_matrix(op, "out", a.out, a.ldo, rows, n, out_type);
@@ -483,7 +488,8 @@ size_t linear_backward_workspace(size_t rows, size_t n, size_t k, int act, bool 
     return plan_backward(JH_BF16, rows, n, k, gated || act != JH_ACT_NONE, !gated).bytes();
 }
 
-void linear_backward(const LinearGradArgs& a, size_t rows, size_t n, size_t k, hipStream_t s) {
+void linear_backward(const LinearGradArgs& args, size_t rows, size_t n, size_t k, hipStream_t s) {
+    LinearGradArgs a = args;
     const char* op = a.gated ? "gated_ffn_backward" : "linear_backward";
     if (a.type == JH_E4M3) refuse(op, "gradients are of bf16 or f16 operands");
     check_sizes(op, a.type, rows, n, k);
@@ -493,6 +499,10 @@ void linear_backward(const LinearGradArgs& a, size_t rows, size_t n, size_t k, h
     const bool keeps_dz = a.gated || a.act != JH_ACT_NONE;
     const int grad_type = a.grad_f32 ? JH_F32 : a.type;
     if (!a.dx && !a.dw && !a.dbias) refuse(op, "no gradient asked for");
+    a.lddy = row_stride(a.lddy, rows, dy_cols);
+    a.ldpre = row_stride(a.ldpre, rows, n);
+    a.ldx = row_stride(a.ldx, rows, k);
+    a.lddx = row_stride(a.lddx, rows, k);
     const BackwardPlan p = plan_backward(a.type, rows, n, k, keeps_dz, a.dbias != nullptr);
     check_workspace(op, a.workspace, a.workspace_bytes, p.bytes());
     const Span ws = span_of(a.workspace, p.bytes(), p.bytes() ? 1 : 0, p.bytes(), JH_E4M3);

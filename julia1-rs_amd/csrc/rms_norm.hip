@@ -496,7 +496,8 @@ int backward_blocks(int rows, int hidden) {
 
 }  // namespace
 
-void rms_norm(const RmsNormArgs& a, hipStream_t s) {
+void rms_norm(const RmsNormArgs& args, hipStream_t s) {
+    RmsNormArgs a = args;
     const char* op = "rms_norm";
     check_width(op, a.hidden);
     if (!plain_type(a.x_type)) refuse(op, "x must be f32, bf16 or f16");
@@ -507,6 +508,7 @@ void rms_norm(const RmsNormArgs& a, hipStream_t s) {
     if ((a.resid == nullptr) != (a.resid_out == nullptr)) refuse(op, "resid and resid_out go together");
     if (a.rows == 0) return;
     const size_t rows = a.rows, h = a.hidden;
+    for (long* ld : {&a.ldx, &a.ldr, &a.ldro, &a.ldo}) *ld = row_stride(*ld, rows, h);
     if (!a.w) refuse(op, "w is null");
     check_matrix(op, "x", a.x, a.ldx, rows, h, a.x_type);
     if (a.resid) {
@@ -538,12 +540,14 @@ void rms_norm(const RmsNormArgs& a, hipStream_t s) {
     HIP_CHECK(hipGetLastError());
 }
 
-void quantize_rows(const RmsNormArgs& a, hipStream_t s) {
+void quantize_rows(const RmsNormArgs& args, hipStream_t s) {
+    RmsNormArgs a = args;
     const char* op = "quantize_rows";
     check_width(op, a.hidden);
     if (!plain_type(a.x_type)) refuse(op, "x must be f32, bf16 or f16");
     if (a.rows == 0) return;
     const size_t rows = a.rows, h = a.hidden;
+    for (long* ld : {&a.ldx, &a.ldo}) *ld = row_stride(*ld, rows, h);
     check_matrix(op, "x", a.x, a.ldx, rows, h, a.x_type);
     check_codes(op, a.out, a.ldo, rows, h);
     if (!a.scales) refuse(op, "scales is null");
@@ -574,6 +578,7 @@ void rms_norm_backward(const RmsNormGradArgs& args, size_t workspace_bytes, hipS
     if ((a.s_type != JH_F32 && a.s_type != a.dy_type) || (a.ds_type != JH_F32 && a.ds_type != a.dy_type))
         refuse(op, "s and ds have dy's type or f32");
     const size_t rows = a.rows, h = a.hidden, need = rms_norm_backward_workspace(a.rows, a.hidden);
+    for (long* ld : {&a.lddy, &a.lds, &a.lddr, &a.ldds}) *ld = row_stride(*ld, rows, h);
     if (a.dw && (!a.partial || ((uintptr_t)a.partial & 15))) refuse(op, "dw needs a 16-byte aligned workspace");
     if (a.dw && workspace_bytes < need) refuse(op, "workspace too small");
     if (rows) {

@@ -492,6 +492,39 @@ def test_gradients_of_no_rows_are_zero():
     assert not bool(dw.any()) and not bool(db.any()) and not bool(dwi.any())
 
 
+@pytest.mark.parametrize("t", [BF16, F16])
+def test_one_row_whatever_its_stride(t):
+    """One row's stride means nothing: a transposed column, whose row stride is 1, gives what a contiguous row gives."""
+    n, k = 96, 200
+    g = gen(31)
+    w, norm_w = randn(g, n, k, std=0.1).to(t), 1 + randn(g, k, std=0.3)
+    x, dy, dh, pre, dres = (randn(g, 1, c).to(t) for c in (k, n, n // 2, n, k))
+    ws = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+
+    def run(row):
+        def empty(c, dtype=t):
+            return row(torch.full((1, c), 7.0, device="cuda").to(dtype))
+
+        x_, dy_, dh_, pre_, dres_ = (row(v) for v in (x, dy, dh, pre, dres))
+        out, kept, dx, h, gu, dxg = empty(n), empty(n), empty(k), empty(n // 2), empty(n), empty(k)
+        y, s, ds, q = empty(k), empty(k), empty(k), empty(k, E4M3)
+        dw, dwg, dnw = torch.empty_like(w), torch.empty(n, k, device="cuda"), torch.empty(k, device="cuda")
+        db, scale, rstd = (torch.empty(c, device="cuda") for c in (n, 1, 1))
+        hip.op_linear(x_, w, out, act="gelu", resid=dy_, pre=kept)
+        hip.op_linear_backward(dy_, x_, w, ws, act="silu", pre=pre_, dx=dx, dw=dw, dbias=db)
+        hip.op_gated_ffn(x_, w, h, gu=gu)
+        hip.op_gated_ffn_backward(dh_, pre_, x_, w, ws, dx=dxg, dw=dwg)
+        hip.op_rms_norm(x_, norm_w, EPS, y, resid=dres_, resid_out=s, rstd=rstd)
+        hip.op_rms_norm_backward(dres_, s, norm_w, rstd, ds, dnw, ws, dres=x_)
+        hip.op_quantize_rows(x_, q, scale)
+        hip.op_linear(x_, w, dy_, resid=dy_.view(1, n))  # in place, by another view of the row
+        torch.cuda.synchronize()
+        return out, kept, dx, dw, db, h, gu, dxg, dwg, y, s, rstd, ds, dnw, q, scale, dy_
+
+    for a, b in zip(run(lambda v: v.clone()), run(lambda v: v.clone().as_strided(v.shape, (1, 1)))):
+        assert torch.equal(a.float(), b.float())
+
+
 # ---------------------------------------------------------------- used together
 
 class Block:
