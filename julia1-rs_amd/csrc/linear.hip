@@ -143,7 +143,7 @@ __global__ __launch_bounds__(THREADS) void split_sum_kernel(const float* partial
 
 unsigned blocks_of(long items, const char* what) {
     const long b = (items + THREADS - 1) / THREADS;
-    if (b > 0x7fffffffL) throw jh_error(JH_ERR_INVALID, std::string(what) + ": too many elements");
+    if (b * THREADS >= 1L << 32) throw jh_error(JH_ERR_INVALID, std::string(what) + ": too many elements");
     return (unsigned)b;
 }
 

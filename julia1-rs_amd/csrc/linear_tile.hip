@@ -184,7 +184,7 @@ template <class T, int LAYOUT, int EPI, int WP, int WQ, int NJ, int KG, int NST>
 void launch_tiles(const LinearArgs& a, hipStream_t s) {
     const long pw = EPI == EPI_GATED ? 32 * WP : 64 * WP, qw = 16 * NJ * WQ;
     const long tiles = ((a.p_cols + pw - 1) / pw) * ((a.q_rows + qw - 1) / qw);
-    if (tiles > 0x7fffffffL) throw jh_error(JH_ERR_INVALID, "linear: too many tiles");
+    if (tiles * 64L * WP * WQ * KG >= 1L << 32) throw jh_error(JH_ERR_INVALID, "linear: too many tiles");
     JH_LAUNCH((linear_tile_kernel<T, LAYOUT, EPI, WP, WQ, NJ, KG, NST>), dim3((unsigned)tiles, (unsigned)a.splits),
               dim3(64 * WP * WQ * KG), 0, s, a);
     HIP_CHECK(hipGetLastError());

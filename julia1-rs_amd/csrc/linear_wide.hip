@@ -184,7 +184,7 @@ template <class T, int LAYOUT, int EPI>
 void launch(const LinearArgs& a, hipStream_t s) {
     const long pw = EPI == EPI_GATED ? TILE / 2 : TILE;
     const long tiles = ((a.p_cols + pw - 1) / pw) * ((a.q_rows + TILE - 1L) / TILE);
-    if (tiles > 0x7fffffffL) throw jh_error(JH_ERR_INVALID, "linear: too many tiles");
+    if (tiles * 512 >= 1L << 32) throw jh_error(JH_ERR_INVALID, "linear: too many tiles");
     JH_LAUNCH((linear_wide_kernel<T, LAYOUT, EPI>), dim3((unsigned)tiles, (unsigned)a.splits), dim3(512), 0, s, a);
     HIP_CHECK(hipGetLastError());
 }

@@ -176,7 +176,7 @@ __device__ inline u32x2 e4m3_codes_half(const float (&p)[8], float a, float inv,
 // One row per TPR threads; NC chunks of 8 values per thread.
 template <int TPR>
 __device__ inline bool row_of(int rows, long& row, int& lane) {
-    row = (long)blockIdx.x * (THREADS / TPR) + threadIdx.x / TPR;
+    row = ((long)blockIdx.y * gridDim.x + blockIdx.x) * (THREADS / TPR) + threadIdx.x / TPR;
     lane = threadIdx.x % TPR;
     return row < rows;
 }
@@ -187,7 +187,7 @@ __global__ __launch_bounds__(THREADS) void rms_norm_kernel(RmsNormArgs a) {
     __shared__ double max_slot[4];
     long row;
     int lane;
-    if (!row_of<TPR>(a.rows, row, lane)) return;  // a whole wave, or (TPR 256) never
+    if (!row_of<TPR>(a.rows, row, lane)) return;  // a whole wave, or (TPR 256) a whole workgroup
     float s[NC][8], w[NC][8];
     {
         Raw8<TX> x[NC];
@@ -442,12 +442,20 @@ void dispatch_row(int hidden, F&& f) {
     }
 }
 
-unsigned row_blocks(int rows, int tpr) { return (unsigned)((rows + THREADS / tpr - 1) / (THREADS / tpr)); }
+int row_blocks(int rows, int tpr) {
+    const int per = THREADS / tpr;
+    return rows / per + (rows % per != 0);
+}
+// A launch holds fewer than 2^32 threads along x: more rows than 2^20 workgroups have go along y.
+dim3 row_grid(int rows, int tpr) {
+    const int b = row_blocks(rows, tpr), x = std::min(b, 1 << 20);
+    return dim3((unsigned)x, (unsigned)((b - 1) / x + 1));
+}
 
 template <class TX, class TR>
 void launch_norm(const RmsNormArgs& a, hipStream_t s) {
     dispatch_row(a.hidden, [&]<int TPR, int NC>() {
-        JH_LAUNCH((rms_norm_kernel<TX, TR, TPR, NC>), dim3(row_blocks(a.rows, TPR)), dim3(THREADS), 0, s, a);
+        JH_LAUNCH((rms_norm_kernel<TX, TR, TPR, NC>), row_grid(a.rows, TPR), dim3(THREADS), 0, s, a);
     });
 }
 template <class TY, class TS, class TD>
@@ -490,8 +498,7 @@ Span vector_span(const float* p, size_t n) { return span_of(p, n, p ? 1 : 0, n, 
 // Workgroups of the backward pass, each with a part of dw: two per CU, fewer where there
 // are fewer rows than they hold at once.
 int backward_blocks(int rows, int hidden) {
-    const int per = THREADS / (hidden <= 2048 ? 64 : 256);
-    return std::max(1, std::min((rows + per - 1) / per, 512));
+    return std::max(1, std::min(row_blocks(rows, hidden <= 2048 ? 64 : 256), 512));
 }
 
 }  // namespace
@@ -557,7 +564,7 @@ void quantize_rows(const RmsNormArgs& args, hipStream_t s) {
     check_disjoint(op, "scales", sc, "x", x);
     check_disjoint(op, "scales", sc, "q", q);
     dispatch_row(a.hidden, [&]<int TPR, int NC>() {
-        const dim3 grid(row_blocks(a.rows, TPR));
+        const dim3 grid = row_grid(a.rows, TPR);
         if (a.x_type == JH_F32) JH_LAUNCH((quantize_rows_kernel<F32, TPR, NC>), grid, dim3(THREADS), 0, s, a);
         else if (a.x_type == JH_BF16) JH_LAUNCH((quantize_rows_kernel<Bf16, TPR, NC>), grid, dim3(THREADS), 0, s, a);
         else JH_LAUNCH((quantize_rows_kernel<F16, TPR, NC>), grid, dim3(THREADS), 0, s, a);
@@ -578,6 +585,7 @@ void rms_norm_backward(const RmsNormGradArgs& args, size_t workspace_bytes, hipS
     if ((a.s_type != JH_F32 && a.s_type != a.dy_type) || (a.ds_type != JH_F32 && a.ds_type != a.dy_type))
         refuse(op, "s and ds have dy's type or f32");
     const size_t rows = a.rows, h = a.hidden, need = rms_norm_backward_workspace(a.rows, a.hidden);
+    if (a.dw && !a.w) refuse(op, "w is null");  // read whatever the number of rows
     for (long* ld : {&a.lddy, &a.lds, &a.lddr, &a.ldds}) *ld = row_stride(*ld, rows, h);
     if (a.dw && (!a.partial || ((uintptr_t)a.partial & 15))) refuse(op, "dw needs a 16-byte aligned workspace");
     if (a.dw && workspace_bytes < need) refuse(op, "workspace too small");

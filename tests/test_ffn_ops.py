@@ -50,6 +50,11 @@ def test_rms_norm_backward_refusals(change):
     assert refused(hip.lib().jh_op_rms_norm_backward, NORM_B, **change)
 
 
+def test_rms_norm_backward_needs_w_without_rows_too():
+    """dw of no rows is zeros, from a kernel that reads w before it knows."""
+    refused(hip.lib().jh_op_rms_norm_backward, NORM_B, rows=0, w=None)
+
+
 QUANT = dict(xt=abi.F32, x=at(0), ldx=64, rows=4, n=64, q=at(1), ldq=64, scales=at(2), stream=None)
 
 
@@ -147,6 +152,8 @@ def test_column_ranges_of_one_buffer_that_share_a_column():
 def test_workspace_sizes():
     assert hip.rms_norm_backward_workspace(1, 64) == 64 * 4
     assert hip.rms_norm_backward_workspace(100000, 4096) == 512 * 4096 * 4
+    for rows in (2**31 - 4, 2**31 - 1):  # the number of workgroups is formed without passing 31 bits
+        assert hip.rms_norm_backward_workspace(rows, 64) == 512 * 64 * 4
     assert hip.linear_backward_workspace(4, 32, 64, "none") < hip.linear_backward_workspace(4, 32, 64, "gelu") + 1
     # the gradient before the activation always has its place
     assert hip.linear_backward_workspace(5000, 1024, 512, "silu") >= 5000 * 1024 * 2

@@ -727,6 +727,28 @@ def test_rows_past_2_31_elements_norms():
     close(out[i], want, r * (gy.abs() * 8 + n.abs() * size * (h + 16)) * 2.0**-24 + want.abs() * half(BF16), "ds")
 
 
+def test_more_rows_than_a_launch_has_along_x():
+    """2^32 threads and more: rows that repeat those of a small call get its bits."""
+    roomy(12)
+    base, h, rows = 4099, 8, 2**26 + 9
+    g = gen(13)
+    few, w = randn(g, base, h).to(BF16), 1 + randn(g, h, std=0.2)
+    x = few.repeat(rows // base + 1, 1)[:rows]
+
+    def run(x):
+        out, q = torch.empty_like(x), torch.empty(x.shape, device="cuda", dtype=E4M3)
+        scales, rstd = (torch.empty(x.shape[0], device="cuda") for _ in range(2))
+        hip.op_rms_norm(x, w, EPS, out, rstd=rstd)
+        hip.op_quantize_rows(x, q, scales)
+        torch.cuda.synchronize()
+        return out.view(torch.int16), q.view(torch.uint8), scales[:, None], rstd[:, None]
+
+    for all_rows, want in zip(run(x), run(few)):
+        whole = rows // base * base
+        assert bool((all_rows[:whole].view(-1, base, want.shape[1]) == want).all())
+        assert torch.equal(all_rows[whole:], want[:rows - whole])
+
+
 def test_rows_past_2_31_elements_products():
     roomy(60)
     rows, n, k = 70000, 32768, 64
