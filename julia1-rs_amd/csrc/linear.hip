@@ -29,7 +29,8 @@ __device__ inline void act_and_grad(float z, int act, float& value, float& grad)
         grad = __builtin_fmaf(z, pdf, cdf);
     } else {
         const float a = act == JH_ACT_SILU ? 1.0f : kTanhA, b = act == JH_ACT_SILU ? 0.0f : kTanhA * kTanhB;
-        const float zz = z * z, s = sigmoid(z * __builtin_fmaf(b, zz, a));
+        // z^2 short of infinity, whose products with 0 (b, or 1 - s) would be NaN
+        const float zz = fminf(z * z, 1e30f), s = sigmoid(z * __builtin_fmaf(b, zz, a));
         value = z * s;
         grad = __builtin_fmaf(value * (1.0f - s), __builtin_fmaf(3.0f * b, zz, a), s);
     }

@@ -131,10 +131,12 @@ __device__ inline void activate(float (&v)[N], int act) {
     } else if (act == JH_ACT_GELU) {
 #pragma unroll
         for (int e = 0; e < N; ++e) v[e] = gelu_erf(v[e]);
-    } else {
-        const float a = act == JH_ACT_SILU ? 1.0f : kTanhA, b = act == JH_ACT_SILU ? 0.0f : kTanhA * kTanhB;
+    } else if (act == JH_ACT_SILU) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) v[e] *= sigmoid(v[e] * __builtin_fmaf(b, v[e] * v[e], a));
+        for (int e = 0; e < N; ++e) v[e] *= sigmoid(v[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] *= sigmoid(v[e] * __builtin_fmaf(kTanhA * kTanhB, v[e] * v[e], kTanhA));
     }
 }
 

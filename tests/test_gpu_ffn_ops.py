@@ -337,6 +337,38 @@ def test_linear_activations(act, rows):
     linear_case(rows, 136, 256, BF16, F32, act, True, True, True, seed=7)
 
 
+@pytest.mark.parametrize("act", ["none", "relu", "gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("rows", [4, 60])
+def test_activations_of_large_values(act, rows):
+    """Values whose squares pass FP32's range: each activation is z or 0 there, its slope 1 or 0 (z^2 itself is inf)."""
+    n, k = 32, 16
+    z = torch.tensor([1e18, 3e19, 2e30, 1e38], device="cuda").repeat_interleave(8)[None, :].repeat(rows, 1)
+    z[1::2] *= -1
+    x = torch.zeros(rows, k, device="cuda", dtype=BF16)
+    out, pre, h = (torch.empty(rows, n, device="cuda", dtype=BF16) for _ in range(3))
+    hip.op_linear(x, torch.zeros(n, k, device="cuda", dtype=BF16), out, bias=z[0].abs().contiguous(), act=act, pre=pre)
+    torch.cuda.synchronize()
+    assert torch.equal(pre, z.abs().to(BF16)) and torch.equal(out, pre)
+    x[:, 0] = z[:, 0].sign().to(BF16)
+    wi = torch.zeros(2 * n, k, device="cuda", dtype=BF16)
+    wi[:n, 0], wi[n:, 0] = z[0].to(BF16), x[0, 0]
+    hip.op_gated_ffn(x, wi, h, act=act)
+    want = torch.where((z > 0) | (act == "none"), z.abs(), torch.zeros_like(z)).to(BF16)
+    torch.cuda.synchronize()
+    assert torch.equal(h, want)
+    pre = z.to(BF16)
+    dy, db = torch.ones(rows, n, device="cuda", dtype=BF16), torch.empty(n, device="cuda")
+    ws = torch.empty(hip.gated_ffn_backward_workspace(rows, n, k) + hip.linear_backward_workspace(rows, n, k, act),
+                     dtype=torch.uint8, device="cuda")
+    hip.op_linear_backward(dy, x, wi[:n], ws, act=act, pre=pre, dbias=db)
+    dwi = torch.empty(2 * n, k, device="cuda")
+    hip.op_gated_ffn_backward(dy, torch.cat([pre, dy], dim=1), x, wi, ws, act=act, dw=dwi)
+    torch.cuda.synchronize()
+    slope = torch.where((z > 0) | (act == "none"), 1.0, 0.0)
+    assert torch.equal(db, slope.sum(dim=0))
+    assert torch.equal(dwi[:n, 0], (slope * z.sign()).sum(dim=0))
+
+
 def test_linear_residual_in_place():
     g = gen(5)
     for rows in (4, 150):
