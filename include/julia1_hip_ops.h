@@ -252,11 +252,16 @@ enum {
  * quantize_rows write: 8), row strides are at most 4 MiB.  f32 vectors
  * (weights of norms, biases, scales, rstd) need 4-byte alignment only.  Feature
  * counts are multiples of 8, or of 16 where they are the contraction of e4m3
- * operands; the number of rows is free, 0 included.  An output may not overlap
- * an input or another output (JH_ERR_INVALID) except where said.  Sums,
+ * operands; the number of rows is free, 0 included (at most 2^30 for products),
+ * and the stride of one row is not used.  An output or a workspace may not overlap
+ * an input or another output (JH_ERR_INVALID) except where said.  Memory is the
+ * current device's, whose stream the call is put on; nothing is allocated, so calls
+ * can be captured into graphs.  A workspace is scratch of one call at a time: calls
+ * that may run at once, replays of graphs among them, have one each.  Sums,
  * statistics and activations are FP32, results are rounded once, and every sum
  * has a fixed order: the same call gives the same bits.  A row's bits may depend
- * on the number of rows in the call (kernels are chosen by size).
+ * on the number of rows in the call (kernels are chosen by size).  Squares are
+ * summed as they are: rows whose sum of squares passes 3.4e38 are not normalised.
  */
 
 /*
@@ -306,7 +311,9 @@ int jh_op_quantize_rows(int x_type, const void* x, size_t ldx, size_t rows, size
  * x_scale[rows] and w_scale[n] belong to e4m3 (NULL: ones); bias f32 [n] or NULL.
  * out and resid (or NULL) have out_type: f32, or type (bf16 for e4m3); resid may
  * be out itself, with its stride.  pre [rows, n] of type (16-bit types; or NULL)
- * receives z for the backward pass.
+ * receives z for the backward pass.  With e4m3 operands and a bf16 output the sums
+ * carry the 8-bit matrix instruction's own error, 1.5e-5 of their norm (1/100 of the
+ * rounding to bf16); with an f32 output they are FP32 sums of exact products.
  */
 int jh_op_linear(int type, const void* x, size_t ldx, const float* x_scale, size_t rows, const void* w,
                  const float* w_scale, size_t n, size_t k, const float* bias, int act, const void* resid,

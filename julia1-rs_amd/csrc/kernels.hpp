@@ -267,5 +267,6 @@ void check_matrix(const char* op, const char* name, const void* p, size_t ld, si
 // the row's length, so that what lies past the row is past the matrix.
 inline long row_stride(long ld, size_t rows, size_t cols) { return rows > 1 ? ld : (long)cols; }
 Span span_of(const void* p, size_t ld, size_t rows, size_t cols, int type);
+Span vector_span(const float* p, size_t n);
 bool spans_overlap(const Span& a, const Span& b);
 void check_disjoint(const char* op, const char* out_name, const Span& out, const char* in_name, const Span& in);

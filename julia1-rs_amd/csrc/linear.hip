@@ -341,6 +341,8 @@ Span span_of(const void* p, size_t ld, size_t rows, size_t cols, int type) {
     return Span{(uintptr_t)p, p ? rows : 0, cols * type_bytes(type), std::max(ld, cols) * type_bytes(type)};
 }
 
+Span vector_span(const float* p, size_t n) { return span_of(p, n, p ? 1 : 0, n, JH_F32); }
+
 // Whether two strided matrices share a byte.  With equal row strides their columns are
 // compared within a row (two column ranges of one buffer do not overlap); otherwise their
 // whole extents are.
@@ -409,6 +411,10 @@ void linear_forward(const LinearArgs& args, size_t rows, size_t n, size_t k, int
     check_disjoint(op, "pre", pre, "w", w);
     check_disjoint(op, "pre", pre, "out", out);
     check_disjoint(op, "pre", pre, "resid", resid);
+    for (const Span& v : {vector_span(a.bias, n), vector_span(a.p_scale, w_rows), vector_span(a.q_scale, rows)}) {
+        check_disjoint(op, "out", out, "the bias or a scale", v);
+        check_disjoint(op, "pre", pre, "the bias or a scale", v);
+    }
     // out may be resid itself: every element is read by the thread that writes it.
     if (a.resid != a.out || a.ldr != a.ldo) check_disjoint(op, "out", out, "resid", resid);
     run(a, s);

@@ -493,8 +493,6 @@ void check_codes(const char* op, const void* q, size_t ld, size_t rows, size_t c
     if (ld > ((size_t)1 << 22)) refuse(op, "the e4m3 output: row stride over 4 MiB");
 }
 
-Span vector_span(const float* p, size_t n) { return span_of(p, n, p ? 1 : 0, n, JH_F32); }
-
 // Workgroups of the backward pass, each with a part of dw: two per CU, fewer where there
 // are fewer rows than they hold at once.
 int backward_blocks(int rows, int hidden) {

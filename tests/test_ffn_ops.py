@@ -82,6 +82,16 @@ def test_linear_refusals(change):
     assert refused(hip.lib().jh_op_linear, LINEAR, **change)
 
 
+def test_outputs_over_the_bias_or_a_scale_are_refused():
+    e4m3 = dict(LINEAR, t=abi.E4M3, pre=None, xs=at(6), ws=at(7), ot=abi.BF16)
+    gated = dict(GATED, t=abi.E4M3, gu=None, xs=at(6), ws=at(7), ldx=64)
+    for change in (dict(bias=at(4)), dict(xs=at(4) + 16), dict(ws=at(4) + 64)):
+        refused(hip.lib().jh_op_linear, e4m3, **change)
+    refused(hip.lib().jh_op_linear, LINEAR, bias=at(5) + 32)
+    for change in (dict(xs=at(2)), dict(ws=at(2) - 24 * 4)):  # the up half's scales
+        refused(hip.lib().jh_op_gated_ffn, gated, **change)
+
+
 def test_linear_in_place_residual_is_not_refused():
     """resid may be out: with no rows such a call does nothing (and needs no device)."""
     args = {**LINEAR, "rows": 0, "out": at(3)}
