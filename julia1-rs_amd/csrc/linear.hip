@@ -163,46 +163,66 @@ long tiles_of(const LinearArgs& a, int p, int q) {
 
 // What a launch of each kernel takes, in us, from its number of tiles and of K steps: a start
 // and an end per round of tiles (launch, first loads, epilogue) and a time per step that grows
-// with the CUs at work (shared L2 and power).  The constants are fits to times of bf16 products
-// on an MI355X (256 CUs; us, the kernel taken in brackets):
+// with the CUs at work (shared L2 and power).  The constants are fits to times of products on an
+// MI355X (256 CUs), the inputs in three sets that take turns, as a layer meets its own; of 86
+// sizes (633 ways to run them) the kernel that comes out cheapest takes 0.3 % longer than the
+// fastest in the mean, 11 % at worst.  Some of them, bf16 (us, the kernel taken in brackets):
 //
-//   rows x n x k         Small   Group   Deep    Pair    256 x 256
-//   512 x 768 x 768      [6.2]   7.5     9.1     11.3    20.6
-//   128 x 1024 x 4096    16.8    [14.5]  28.3    36.6    69.1
-//   1024 x 1024 x 4096   [19.1]  21.1    29.2    46.4    69.8
-//   1024 x 4096 x 1024   17.5    26.3    [13.4]  15.6    25.4
-//   2048 x 4096 x 4096   105     147     73.0    [60.3]  71.8
-//   4096 x 4096 x 4096   203     291     140     117     [96.3]
-//   9482 x 4096 x 1024   149     246     108     88.7    [81.9]
-enum { SMALL, GROUP, DEEP, PAIR, WIDE, KERNELS };
-constexpr double CUS = 256;
+//   rows x n x k              Small   Group   Deep    Pair    Tall    256 x 256
+//   512 x 768 x 768           [7.0]           9.9     12.2    13.8    21.2
+//   1024 x 1024 x 4096        [19.9]          30.4    51.3    45.1    70.7
+//   1024 x 4096 x 1024        19.5            [14.3]  19.4    18.4    26.2
+//   9482 x 768 x 1152         32.3            27.1    25.4    [21.8]  29.6
+//   2048 x 4096 x 4096        111             71.6    68.6    [59.9]  74.9
+//   4096 x 4096 x 4096        204             143     135     121     [101]
+//   9482 x 4096 x 1024        147             111     99.8    96.6    [88.3]
+//   dx of 1024 x 4096 x 1024  25.5    [22.3]  37.7    50.7            78.4
+//   dx of 9482 x 2304 x 768   70.1    91.0    48.2    [37.4]          50.0
+//   dw of 4096 x 4096 x 1024  66.1    78.7    [40.0]  50.2            98.2
+//   dw of 8192 x 4096 x 4096  527     742     340     264             [223]
+enum { SMALL, GROUP, DEEP, PAIR, TALL, WIDE, KERNELS };
+constexpr long CUS = 256;
 
 double cost(int kernel, const LinearArgs& a, long splits) {
     const double s = (double)((steps_of(a) + splits - 1) / splits);
-    auto rounds = [](double t, double slots) { return std::ceil(t / slots); };
-    auto load = [](double t) { return std::min(1.0, t / CUS); };
+    const bool by_cols = a.layout != ROWS_ROWS;
+    // `of(n)`: a round of n tiles, `slots` of which the GPU holds
+    auto rounds = [](long t, long slots, auto of) {
+        return (double)(t / slots) * of((double)slots) + (t % slots ? of((double)(t % slots)) : 0.0);
+    };
+    auto load = [](double t) { return std::min(1.0, t / (double)CUS); };
     switch (kernel) {
         case SMALL: {
-            const double t = (double)(tiles_of(a, 64, 64) * splits);
-            return t <= CUS ? 3.0 + 0.22 * s : rounds(t, 2 * CUS) * (0.42 * s + 2.0) + 1.0;
+            const long t = tiles_of(a, 64, 64) * splits;
+            if (t <= CUS) return 3.7 + (by_cols ? 0.33 : 0.215 + 0.05 * load((double)t)) * s;
+            return rounds(t, 2 * CUS, [&](double) { return 0.42 * s + 2.0; }) + (by_cols ? 5.0 : 1.0);
         }
         case GROUP: {
-            const double t = (double)(tiles_of(a, 64, 64) * splits);
-            return rounds(t, CUS) * (std::ceil(s / 4) * (t <= 64 ? 0.58 : 0.98) + 3.5) + 1.5;
+            const long t = tiles_of(a, 64, 64) * splits;
+            return rounds(t, CUS, [&](double) { return std::ceil(s / 4) + 5.0; }) + 1.5;
         }
         case DEEP: {
-            const double t = (double)(tiles_of(a, 128, 128) * splits);
-            // transposing reads move half as much per instruction, and this kernel waits for LDS most
-            const double by_cols = a.layout == COLS_COLS ? 1.4 : a.layout == COLS_ROWS ? 1.15 : 1.0;
-            return rounds(t, CUS) * (s * (0.35 + 0.19 * load(t)) * by_cols + 3.0) + 1.0;
+            const long t = tiles_of(a, 128, 128) * splits;
+            // operands well past the L2s' 32 MB come late for its two steps per group in flight (dw of
+            // 9482 x 1024 x 4096, 97 MB, in one part: 83 us of inputs read just before, 104 of others;
+            // Pair in two parts 92 and 99.  9482 x 1024 x 768, 34 MB, in four parts: 35 and 35)
+            const double far = ((double)a.q_rows + a.p_cols) * a.k * 2 > 48e6 ? 0.13 : 0.0;
+            if (by_cols) return rounds(t, CUS, [&](double n) { return s * (0.49 + (0.05 + far) * load(n)) + 4.0; }) + 1.0;
+            return rounds(t, CUS, [&](double n) { return s * (0.35 + 0.19 * load(n)) + 3.0; }) + 1.5;
         }
         case PAIR: {
-            const double t = (double)(tiles_of(a, 128, 128) * splits);
-            return rounds(t, 2 * CUS) * (s * (t <= CUS ? 0.65 : 0.88) + 3.5) + 1.0;
+            const long t = tiles_of(a, 128, 128) * splits;
+            return rounds(t, 2 * CUS, [&](double n) { return s * (n > CUS ? 0.92 : 0.62 + 0.16 * load(n)) + 5.0; }) + 1.0;
+        }
+        case TALL: {
+            const long t = tiles_of(a, 128, 256) * splits;
+            return rounds(t, CUS, [&](double n) { return s * (0.54 + 0.33 * load(n)) + 4.2; }) + 2.5;
         }
         default: {
-            const double t = (double)(tiles_of(a, 256, 256) * splits);
-            return rounds(t, CUS) * (s * (1.0 + 0.4 * load(t)) + 6.0) + 1.0;
+            const long t = tiles_of(a, 256, 256) * splits;
+            const double alone = a.layout == COLS_COLS ? 1.37 : by_cols ? 1.0 : 0.88;
+            const double all = a.layout == COLS_COLS ? 1.57 : by_cols ? 1.45 : 1.37;
+            return rounds(t, CUS, [&](double n) { return s * (alone + (all - alone) * load(n) * load(n)) + 9.0; }) + 1.0;
         }
     }
 }
@@ -223,9 +243,15 @@ Choice pick(const LinearArgs& a, bool gradient) {
     const double out = (double)a.q_rows * a.p_cols * 4;
     for (long splits = 1; splits <= (gradient ? MAX_SPLITS : 1); splits += splits < 4 ? 1 : splits < 8 ? 2 : 4) {
         if (splits > 1 && (steps_of(a) < splits * MIN_STEPS || out * splits > split_bytes(a))) break;
-        const double sum = splits > 1 ? 2.5 + (2 * splits + 0.5) * out / 4.5e6 : 0.0;  // written and read
+        const double sum = splits > 1 ? 2.5 + (2 * splits + 0.5) * out / 5e6 : 0.0;  // written and read
         for (int kernel = 0; kernel < KERNELS; ++kernel) {
-            if (kernel == WIDE && a.type == JH_E4M3 && a.out_f32) continue;  // has no bf16 fragments of e4m3
+            // no room there for e4m3 fragments widened to bf16; Tall gains nothing by columns (9482 x 768
+            // x 2304: 38.2 us, Pair 37.5)
+            if (kernel >= TALL && a.type == JH_E4M3 && a.out_f32) continue;
+            if (kernel == TALL && a.layout != ROWS_ROWS) continue;
+            // The groups share a long contraction; k contiguous that gains only where both operands are
+            // in L2 already (128 x 1024 x 4096: 15.1 us against Small's 17.5, else 20.0 against 17.7)
+            if (kernel == GROUP && a.layout == ROWS_ROWS) continue;
             const double c = cost(kernel, a, splits) + sum;
             if (c < best.cost) best = {kernel, (int)splits, c};
         }
@@ -247,12 +273,13 @@ LinearArgs row_range(const LinearArgs& a, int r0, int rows) {
 }
 
 // Rows that 256 x 256 tiles take in whole rounds of the CUs, where that and another kernel
-// for the rest come cheaper than any kernel alone; else 0.  9482 x 4096 x 1024 (608 tiles, 2.4
-// rounds): 7936 rows in two rounds, the rest in one of 128 x 128 tiles.
+// for the rest come cheaper than any kernel alone; else 0.  18000 x 1024 x 4096 (284 tiles): 164
+// us at once, 127 as 16384 rows and 1616 on 64 x 64 tiles; 5000 x 4096 x 4096: 161 and 138; with a
+// last round half full it is even (9482 x 2304 x 768: 46.5 and 47.4).
 int whole_rounds(const LinearArgs& a, double alone) {
     if (a.type == JH_E4M3 && a.out_f32) return 0;
-    const long across = tiles_of(row_range(a, 0, 1), 256, 256), rounds = tiles_of(a, 256, 256) / (long)CUS;
-    const long rows = rounds * (long)CUS / across * 256;
+    const long across = tiles_of(row_range(a, 0, 1), 256, 256), rounds = tiles_of(a, 256, 256) / CUS;
+    const long rows = rounds * CUS / across * 256;
     if (rows <= 0 || rows >= a.q_rows) return 0;
     const double c = cost(WIDE, row_range(a, 0, (int)rows), 1) +
                      pick(row_range(a, (int)rows, a.q_rows - (int)rows), false).cost;
@@ -267,7 +294,7 @@ long partial_bytes(const LinearArgs& a) {
 void launch(int kernel, const LinearArgs& a, hipStream_t s) {
     if (kernel == WIDE) launch_linear_wide(a, s);
     else launch_linear_tile(a, kernel == SMALL ? LinearTile::Small : kernel == GROUP ? LinearTile::Group
-                               : kernel == DEEP ? LinearTile::Deep : LinearTile::Pair, s);
+                               : kernel == DEEP ? LinearTile::Deep : kernel == PAIR ? LinearTile::Pair : LinearTile::Tall, s);
 }
 
 template <class T>

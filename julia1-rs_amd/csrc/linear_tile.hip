@@ -4,10 +4,16 @@
 //
 //   Small  64 x 64, 4 waves, 4 stages (64 KB)
 //   Group  64 x 64, 4 groups of 4 waves, 2 stages (128 KB): a quarter of the steps, one
-//          after the other, for few tiles of long contractions
-//   Deep   128 x 128, 8 waves, 4 stages (128 KB): one tile per CU
+//          after the other, for few tiles of long contractions by columns
+//   Deep   128 x 128, one tile per CU (128 KB): 8 waves and 4 stages where k is contiguous;
+//          2 groups of 4 waves and 2 stages where an operand lies by columns, as a transposing
+//          read brings half as much and waves of 64 x 64 read less (a contraction of 9482 into
+//          1024 x 4096: 100 us with 8 waves, 84 with the groups; k contiguous, 1024 x 4096 x
+//          4096: 37 and 40)
 //   Pair   128 x 128, 4 waves, 2 stages (64 KB): two workgroups per CU, one's epilogue and
 //          waits under the other's MFMAs
+//   Tall   128 (P) x 256 (Q), 8 waves, 3 stages (144 KB), k contiguous: three quarters of
+//          Pair's operand bytes
 //
 // Where each is taken, and what it measured, stands at pick() in linear.hip.
 #include <hip/hip_runtime.h>
@@ -193,9 +199,12 @@ void launch_tiles(const LinearArgs& a, hipStream_t s) {
 template <class T, int LAYOUT, int EPI>
 void launch(const LinearArgs& a, LinearTile tile, hipStream_t s) {
     if (tile == LinearTile::Small) launch_tiles<T, LAYOUT, EPI, 1, 4, 1, 1, 4>(a, s);
-    else if (tile == LinearTile::Group) launch_tiles<T, LAYOUT, EPI, 1, 4, 1, 4, 2>(a, s);
-    else if (tile == LinearTile::Deep) launch_tiles<T, LAYOUT, EPI, 2, 4, 2, 1, 4>(a, s);
-    else launch_tiles<T, LAYOUT, EPI, 2, 2, 4, 1, 2>(a, s);
+    else if (tile == LinearTile::Pair) launch_tiles<T, LAYOUT, EPI, 2, 2, 4, 1, 2>(a, s);
+    else if constexpr (LAYOUT != ROWS_ROWS) {
+        if (tile == LinearTile::Group) launch_tiles<T, LAYOUT, EPI, 1, 4, 1, 4, 2>(a, s);
+        else launch_tiles<T, LAYOUT, EPI, 2, 2, 4, 2, 2>(a, s);
+    } else if (std::is_same_v<T, E4m3Wide> || tile == LinearTile::Deep) launch_tiles<T, LAYOUT, EPI, 2, 4, 2, 1, 4>(a, s);
+    else if constexpr (!std::is_same_v<T, E4m3Wide>) launch_tiles<T, LAYOUT, EPI, 2, 4, 4, 1, 3>(a, s);
 }
 
 }  // namespace

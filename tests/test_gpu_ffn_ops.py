@@ -306,9 +306,10 @@ def test_linear(rows, n, k, t, out_t):
                 t != E4M3 and i % 4 < 2, seed=100 + i)
 
 
-# one size for each kernel that larger products run on: 128 x 128 tiles one to a CU and two to a CU, 256 x 256 tiles,
-# those for whole rounds of the CUs with the rest on smaller ones, and 64 x 64 tiles whose waves share a long contraction
-KERNELS = [(1000, 4000, 520), (1500, 4000, 520), (3900, 4000, 520), (4700, 4000, 520), (129, 264, 4104)]
+# sizes for each kernel that larger products run on: 128 x 128 tiles one to a CU and two to a CU, 128 x 256 tiles, 256 x 256
+# tiles, those for whole rounds of the CUs with the rest on smaller ones, and 64 x 64 tiles of a long contraction
+KERNELS = [(1000, 4000, 520), (1500, 4000, 520), (1600, 4704, 520), (1500, 4000, 2080), (3900, 4000, 520),
+           (4700, 4000, 520), (129, 264, 4104)]
 
 
 @pytest.mark.parametrize("rows,n,k", KERNELS)
@@ -323,9 +324,11 @@ def test_gated_ffn_kernels(rows, n, k, t):
     test_gated_ffn(rows, n // 16 * 8, k, t)
 
 
-# the same for both gradients (dx: rows x k over n; dw: n x k over rows), and contractions that are cut into parts
+# the same for both gradients (dx: rows x k over n; dw: n x k over rows), contractions that are cut into parts, and 64 x 64
+# tiles whose waves share a long contraction
 @pytest.mark.parametrize("rows,n,k", [(1500, 520, 4000), (3900, 520, 4000), (4700, 520, 4000), (520, 1504, 4000),
-                                      (520, 3904, 4000), (520, 4704, 4000), (9000, 1032, 776), (264, 6008, 264)])
+                                      (520, 3904, 4000), (520, 4704, 4000), (9000, 1032, 776), (264, 6008, 264),
+                                      (1000, 3600, 1000), (3600, 1000, 1000), (7000, 1032, 776)])
 @pytest.mark.parametrize("t,grad_t", [(BF16, BF16), (F16, F32)])
 def test_linear_backward_kernels(rows, n, k, t, grad_t):
     test_linear_backward(rows, n, k, t, grad_t, "gelu")
