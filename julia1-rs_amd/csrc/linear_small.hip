@@ -1,7 +1,12 @@
 // Linear and gated projections of up to 16 rows: W streams from memory straight into
 // registers, once.  A workgroup of eight waves computes 16 output columns (their gate and up
 // rows when gated); its waves take pieces of K in turn, several loads in flight, and their sums
-// are added through LDS in wave order.
+// are added through LDS in wave order.  MFMA does the products because the rows come for free
+// there, not for its rate; x is read by every workgroup, from L2.
+//
+// Bound by latency while W is small (a launch is 2 us; W's first bytes come 2 us later): 8 x 1152
+// x 768 gated, 3.5 MB, 5.0 us; 1 x 768 x 1152, 1.8 MB, 4.1 us; then by memory: 16 x 4096 x 4096,
+// 34 MB, 10.1 us (3.3 TB/s).
 #include <hip/hip_runtime.h>
 
 #include "linear.hpp"

@@ -4,6 +4,16 @@
 // All are one pass over memory: a row is held in registers, 8 values per chunk and lane,
 // between the reduction over it and its use.  Rows of up to 2048 values belong to one
 // wavefront (four rows per workgroup), longer ones (up to 16384) to a workgroup of four.
+// What bounds them is the memory (a copy of 1 GiB: 5.1 TB/s), on an MI355X:
+//
+//   rms_norm           9482 x 1024, bf16 + f32 residual -> e4m3     107 MB   23.3 us  4.6 TB/s
+//   rms_norm           1 x 768                                                2.2 us  (a launch)
+//   quantize_rows      8192 x 8192 f32                              336 MB   62.9 us  5.3 TB/s
+//   quantize_rows      9482 x 1152 bf16                              33 MB    9.3 us  3.5 TB/s (1)
+//   rms_norm_backward  16384 x 4096 bf16, with dres and dw          537 MB   98.5 us  5.4 TB/s
+//   column_sum         512 x 4096, of that dw's parts                 8 MB    4.9 us
+//
+//   (1) a launch (2 us) and the codes' arithmetic count here: 12.7 us with codes formed in 64 bits
 //
 //   forward   s = x + resid, rounded to the residual's type (what is stored is what is
 //             normalised); r = 1 / sqrt(mean(s^2) + eps); y = s r w
@@ -153,8 +163,7 @@ __device__ inline u32x2 e4m3_codes(const double (&p)[8], double a, double inv) {
 // correctly rounded quotient of n by a (a product with the reciprocal, corrected once), and the
 // sign of its remainder, exact too, says on which side of q1 the quotient itself lies.  That
 // makes the float rounded to odd.  `lift` (a power of two) keeps the remainder
-// normal and n finite where the row's maximum is far from 1.  (9482 x 1152 bf16: 12.7 us in 64
-// bits, bound by arithmetic.)
+// normal and n finite where the row's maximum is far from 1.
 __device__ inline u32x2 e4m3_codes_half(const float (&p)[8], float a, float inv, float lift) {
     uint32_t h[4];
 #pragma unroll
@@ -299,8 +308,8 @@ __global__ __launch_bounds__(THREADS) void quantize_rows_kernel(RmsNormArgs a) {
 }
 
 // Workgroups walk the rows in strides of the grid and keep their part of dw in registers;
-// the parts (one per workgroup) are added by column_sum_kernel.  TPR 64: the four waves'
-// parts are first joined through LDS, in wave order.
+// the parts (one per workgroup, so at most 512) are added by column_sum_kernel: no atomics, the
+// same sum every time.  TPR 64: the four waves' parts are first joined through LDS, in wave order.
 template <class TY, class TS, class TD, int TPR, int NC>
 __global__ __launch_bounds__(THREADS) void rms_norm_backward_kernel(RmsNormGradArgs a) {
     constexpr int RPB = THREADS / TPR;
@@ -392,7 +401,7 @@ __global__ __launch_bounds__(THREADS) void rms_norm_backward_kernel(RmsNormGradA
 
 // out[c] = sum over r of in[r, c] in FP32: a workgroup owns 64 columns, four per lane of 16,
 // and its 64 groups of 16 lanes each add a run of rows, eight loads in flight; the groups' sums
-// are added in group order.
+// are added in group order.  Bound by latency: 500 x 1024 takes 4.7 us, of which a launch is 2.
 constexpr int SUM_THREADS = 1024, SUM_GROUPS = SUM_THREADS / 16;
 __global__ __launch_bounds__(SUM_THREADS) void column_sum_kernel(const float* in, int rows, int cols, float* out) {
     __shared__ __align__(16) float part[SUM_GROUPS][64];
