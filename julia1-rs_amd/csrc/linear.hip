@@ -49,8 +49,8 @@ __device__ inline void load8_of(const void* p, float (&v)[8]) {
 // dz = dy act'(pre) (rounded to T) and the column sums of its unrounded values, a part per
 // blockIdx.y.  A lane owns 8 columns, the four waves of a workgroup every fourth of its rows;
 // their sums are joined in wave order.  dz is kept because both products read it, one of them by
-// columns.  Bound by memory: 9482 x 1024 bf16 gelu, 58 MB, takes 16.7 us (3.5 TB/s; 21.2 with four
-// rows in flight per wave).
+// columns.  Bound by memory: 9482 x 1024 bf16 gelu, 58 MB, takes 18 us (3.2 TB/s; 21 with four rows
+// in flight per wave).
 template <class T>
 __global__ __launch_bounds__(THREADS) void act_grad_kernel(ActGradArgs a) {
     __shared__ float join[4][64][9];
