@@ -4,10 +4,11 @@
 //
 // Measured (MFMA busy and clock from counters): 16384 x 8192 x 2048 bf16 gated with silu, 1.10
 // PFLOP in 917 us (1.20 PFLOP/s, busy 59 % at 1.93 GHz: power holds the clock there, 2.4 GHz at
-// rest); 8192 x 4096 x 4096 e4m3, 275 GFLOP in 127 us (2.17 PFLOP/s, busy 43 % at 2.1 GHz: a step's
-// 64 KB take as long to come in, at 64 bytes a cycle and CU, as its MFMAs); 8192^3 bf16 0.92 ms
-// (1.19 PFLOP/s; by columns 1.29 for dx, 1.19 for dw).  LDS is read a fifth of the time, without
-// bank conflicts.
+// rest); 8192^3 bf16 0.92 ms (1.19 PFLOP/s; by columns 1.29 for dx, 1.19 for dw); 4096^3 e4m3 57 us
+// (2.40 PFLOP/s); 8192 x 4096 x 4096 e4m3 with bias, silu and residual 127 us (2.17), whose tiles
+// end together twice: 67 MB of residuals and outputs in a burst, 13 of 63 us at the memory's rate.
+// LDS is read a fifth of the time, without bank conflicts; a step's 64 KB of operands take half as
+// long to come in as its MFMAs (2048 cycles), all CUs reading.
 //
 // A K step runs in four phases, each a quadrant of the wave's block: 32 P rows by 64 Q rows,
 // 16 MFMAs of 16 bits.  A phase first reads the fragments that it or the next lacks and
