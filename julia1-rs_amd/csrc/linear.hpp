@@ -272,6 +272,72 @@ __device__ inline void store16(void* dst, const float (&v)[N]) {
                                               T::pack(v[c + 4], v[c + 5]), T::pack(v[c + 6], v[c + 7])};
 }
 
+// The stores' layout.  Of a block of 16 rows a lane of the accumulators holds 16 columns of row
+// lane % 16, four lanes 64 columns of it.  Lanes exchange 16-byte runs so that an instruction
+// covers whole 128-byte lines: 8 rows of 128 bytes in 16 bits, 4 rows of 256 in FP32.  (16 rows
+// of 64 bytes or of every other run keep the memory path busy for longer: 16384 x 4096 x 512 bf16
+// took 98.5 us so and takes 84.8, the FP32 parts of dw of 9482 x 2304 x 768 51.6 and 48.1.)  The
+// exchange is its own inverse: residuals are loaded in whole lines as well.
+//
+// Lane bit 3 (2) changes places with which of two runs it is.
+__device__ __forceinline__ void exchange_halves(u32x4& a, u32x4& b) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int x = (int)a[i], y = (int)b[i];
+        a[i] = (uint32_t)__builtin_amdgcn_update_dpp(x, y, 0x128, 0xf, 0xc, false);  // rotated by 8, into lanes 8 .. 15
+        b[i] = (uint32_t)__builtin_amdgcn_update_dpp(y, x, 0x128, 0xf, 0x3, false);  // into lanes 0 .. 7
+    }
+}
+__device__ __forceinline__ void exchange_quarters(u32x4& a, u32x4& b) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int x = (int)a[i], y = (int)b[i];
+        a[i] = (uint32_t)__builtin_amdgcn_update_dpp(x, y, 0x124, 0xf, 0xa, false);  // rotated by 4, into lanes 4 .. 7 and 12 .. 15
+        b[i] = (uint32_t)__builtin_amdgcn_update_dpp(y, x, 0x12c, 0xf, 0x5, false);  // by 12, into the others
+    }
+}
+__device__ __forceinline__ void exchange(u32x4 (&v)[2]) { exchange_halves(v[0], v[1]); }
+__device__ __forceinline__ void exchange(u32x4 (&v)[4]) {
+    exchange_halves(v[0], v[2]);
+    exchange_halves(v[1], v[3]);
+    exchange_quarters(v[0], v[1]);
+    exchange_quarters(v[2], v[3]);
+}
+// Where run `i` of N lies for a lane after the exchange: its row of the block, and its column
+// past the lane's first.
+template <int N>
+__device__ inline int line_row(int i, int lane) { return (lane & (16 / N - 1)) + 16 / N * i; }
+template <int N>
+__device__ inline int line_col(int lane) { return (lane & 15) / (16 / N) * (16 / N); }
+
+// A block's rows t0 .., columns c .. of the lane's four: to memory, of elements of 32 / N bytes.
+template <int N>
+__device__ __forceinline__ void store_lines(void* out, long ld, long t0, int c, int lane, int rows, int cols, u32x4 (&v)[N]) {
+    exchange(v);
+    const int at = c + line_col<N>(lane);
+    if (at >= cols) return;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const long t = t0 + line_row<N>(i, lane);
+        if (t < rows) *(u32x4*)((uint8_t*)out + (t * ld + at) * N) = v[i];
+    }
+}
+template <class T>
+__device__ __forceinline__ void store_half(void* out, long ld, long t0, int c, int lane, int rows, int cols, const float (&z)[2][8]) {
+    u32x4 v[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        v[h] = u32x4{T::pack(z[h][0], z[h][1]), T::pack(z[h][2], z[h][3]), T::pack(z[h][4], z[h][5]), T::pack(z[h][6], z[h][7])};
+    store_lines<2>(out, ld, t0, c, lane, rows, cols, v);
+}
+__device__ __forceinline__ void store_f32(void* out, long ld, long t0, int c, int lane, int rows, int cols, const float (&z)[2][8]) {
+    u32x4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        v[i] = __builtin_bit_cast(u32x4, f32x4{z[i >> 1][4 * (i & 1)], z[i >> 1][4 * (i & 1) + 1], z[i >> 1][4 * (i & 1) + 2], z[i >> 1][4 * (i & 1) + 3]});
+    store_lines<4>(out, ld, t0, c, lane, rows, cols, v);
+}
+
 // What the epilogue needs of eight output columns, whatever the row: loaded once per lane.
 template <class T>
 struct ColumnTerms {
@@ -295,53 +361,47 @@ struct ColumnTerms {
     }
 };
 
-// The residual of eight columns of one row, raw (e4m3 operands with FP32 outputs are E4m3Wide).
+// The residual of a block's 16 rows and the lane's 16 columns, as loaded (e4m3 operands with FP32
+// outputs are E4m3Wide).
 template <class T>
-struct Resid8 {
+struct ResidLines {
     static constexpr bool HALF_ONLY = __is_same(T, E4m3);
-    u32x4 v[HALF_ONLY ? 1 : 2];
-    __device__ void load(const LinearArgs& a, long t, int c0) {
-        const long at = min(t, (long)a.q_rows - 1) * a.ldr + min(c0, a.p_cols - 8);
-        if (!HALF_ONLY && a.out_f32) {
-            v[0] = *(const u32x4*)((const float*)a.resid + at);
-            v[HALF_ONLY ? 0 : 1] = *(const u32x4*)((const float*)a.resid + at + 4);
-        } else {
-            v[0] = *(const u32x4*)((const uint16_t*)a.resid + at);
+    u32x4 v[HALF_ONLY ? 2 : 4];
+    // Rows and columns past the last are read as the last.
+    __device__ __forceinline__ void load(const LinearArgs& a, long t0, int c, int lane) {
+        const bool f32 = !HALF_ONLY && a.out_f32;
+        const int run = f32 ? 4 : 8, at = min(c + (f32 ? line_col<4>(lane) : line_col<2>(lane)), a.p_cols - run);
+#pragma unroll
+        for (int i = 0; i < (HALF_ONLY ? 2 : 4); ++i) {
+            const long t = min(t0 + (lane & (run - 1)) + run * i, (long)a.q_rows - 1);
+            if (i < 2 || f32) v[i] = *(const u32x4*)((const uint8_t*)a.resid + (t * a.ldr + at) * (f32 ? 4 : 2));
+        }
+    }
+    __device__ __forceinline__ void add_half(float (&z)[2][8]) const {
+        u32x4 r[2] = {v[0], v[1]};
+        exchange(r);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                z[h][2 * e] += T::lo(r[h][e]);
+                z[h][2 * e + 1] += T::hi(r[h][e]);
+            }
+    }
+    __device__ __forceinline__ void add_f32(float (&z)[2][8]) const {
+        if constexpr (!HALF_ONLY) {
+            u32x4 r[4] = {v[0], v[1], v[2], v[3]};
+            exchange(r);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t u = r[i][e];
+                    z[i >> 1][4 * (i & 1) + e] += __builtin_bit_cast(float, u);
+                }
         }
     }
 };
-
-// Eight columns of one output row from their sums z: c0 .. c0+7.
-template <class T>
-__device__ inline void finish8(const LinearArgs& a, float (&z)[8], long t, int c0, float qs, const ColumnTerms<T>& col,
-                               const Resid8<T>& resid) {
-    col.apply(a, z, qs);
-    if constexpr (T::bytes == 2)
-        if (a.pre) store16<T>((uint16_t*)a.pre + t * a.ldpre + c0, z);
-    activate(z, a.act);
-    if (!Resid8<T>::HALF_ONLY && a.out_f32) {
-        if (a.resid) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint32_t r = resid.v[Resid8<T>::HALF_ONLY ? 0 : e >> 2][e & 3];
-                z[e] += __builtin_bit_cast(float, r);
-            }
-        }
-        float* o = (float*)a.out + t * a.ldo + c0;
-        *(f32x4*)o = f32x4{z[0], z[1], z[2], z[3]};
-        *(f32x4*)(o + 4) = f32x4{z[4], z[5], z[6], z[7]};
-    } else {
-        if (a.resid) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t r = resid.v[0][e];
-                z[2 * e] += T::lo(r);
-                z[2 * e + 1] += T::hi(r);
-            }
-        }
-        store16<T>((uint16_t*)a.out + t * a.ldo + c0, z);
-    }
-}
 
 // Eight columns of one row of the gated projections: g their gate, u their up part.
 template <class T>
@@ -373,14 +433,15 @@ struct Epilogue {
     const LinearArgs& a;
     int t0, c0, lane;
     ColumnTerms<T> col[2];
-    Resid8<T> resid[AHEAD][2];
+    ResidLines<T> resid[AHEAD];
     float scale[NJ];  // of e4m3 rows
 
     __device__ Epilogue(const LinearArgs& args, int row0, int col0, int lane_id) : a(args), t0(row0), lane(lane_id) {
         const int g = lane >> 4;
         c0 = col0 + (HALF < NJ && LAYOUT != ROWS_ROWS ? (g & 1) * 16 + (g >> 1) * 128 : g * (EPI == EPI_GATED ? 8 : 16));
     }
-    __device__ int row(int j) const { return t0 + (j < HALF ? j * 16 : 128 + (j - HALF) * 16) + (lane & 15); }
+    __device__ int first_row(int j) const { return t0 + (j < HALF ? j * 16 : 128 + (j - HALF) * 16); }
+    __device__ int row(int j) const { return first_row(j) + (lane & 15); }
     __device__ void load_columns() {
         if (a.partial) return;
         col[0].load(a, c0, a.p_scale);
@@ -395,9 +456,7 @@ struct Epilogue {
         if (EPI == EPI_GATED || !a.resid) return;
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                if (j + i < NJ) resid[i][h].load(a, row(j + i), c0 + 8 * h);
+            if (j + i < NJ) resid[i].load(a, first_row(j + i), c0, lane);
     }
     __device__ void start() {
         if constexpr (EARLY) {
@@ -414,32 +473,36 @@ struct Epilogue {
             if constexpr (LAYOUT != ROWS_ROWS) transpose_groups(c);
             const long t = row(j);
             const float qs = T::bytes == 1 ? scale[j] : 1.0f;
-            if (t < a.q_rows) {
-                if constexpr (EPI == EPI_GATED) {
-                    float ga[8], up[8];
+            if constexpr (EPI == EPI_LINEAR) {
+                float z[2][8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        ga[e] = c[e >> 2][e & 3];
-                        up[e] = c[2 + (e >> 2)][e & 3];
-                    }
-                    if (c0 < a.p_cols) finish_gated8<T>(a, ga, up, t, c0, qs, col[0], col[1]);
+                for (int e = 0; e < 16; ++e) z[e >> 3][e & 7] = c[e >> 2][e & 3];
+                const long first = first_row(j);
+                if (a.partial) {
+                    store_f32(a.partial + (long)split * a.q_rows * a.p_cols, a.p_cols, first, c0, lane, a.q_rows, a.p_cols, z);
                 } else {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int ch = c0 + 8 * h;
-                        if (ch >= a.p_cols) continue;
-                        if (a.partial) {
-                            float* o = a.partial + ((long)split * a.q_rows + t) * a.p_cols + ch;
-                            *(f32x4*)o = c[2 * h];
-                            *(f32x4*)(o + 4) = c[2 * h + 1];
-                        } else {
-                            float z[8];
+                    for (int h = 0; h < 2; ++h) col[h].apply(a, z[h], qs);
+                    if constexpr (T::bytes == 2)
+                        if (a.pre) store_half<T>(a.pre, a.ldpre, first, c0, lane, a.q_rows, a.p_cols, z);
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) z[e] = c[2 * h + (e >> 2)][e & 3];
-                            finish8<T>(a, z, t, ch, qs, col[h], resid[j % AHEAD][h]);
-                        }
+                    for (int h = 0; h < 2; ++h) activate(z[h], a.act);
+                    if (!ResidLines<T>::HALF_ONLY && a.out_f32) {
+                        if (a.resid) resid[j % AHEAD].add_f32(z);
+                        store_f32(a.out, a.ldo, first, c0, lane, a.q_rows, a.p_cols, z);
+                    } else {
+                        if (a.resid) resid[j % AHEAD].add_half(z);
+                        store_half<T>(a.out, a.ldo, first, c0, lane, a.q_rows, a.p_cols, z);
                     }
                 }
+            } else if (t < a.q_rows && c0 < a.p_cols) {
+                float ga[8], up[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    ga[e] = c[e >> 2][e & 3];
+                    up[e] = c[2 + (e >> 2)][e & 3];
+                }
+                finish_gated8<T>(a, ga, up, t, c0, qs, col[0], col[1]);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -454,8 +517,8 @@ __device__ inline void tile_coords(int b, int n_p, int n_q, int& tp, int& tq) {
     const int ntiles = n_p * n_q, xcd = b & 7, q8 = ntiles >> 3, r8 = ntiles & 7;
     const int tile = xcd * q8 + (xcd < r8 ? xcd : r8) + (b >> 3);
     const int grp = tile / (GROUP * n_p), gi = tile - grp * GROUP * n_p, gh = min(GROUP, n_q - grp * GROUP);
-    tp = gi / gh;
-    tq = grp * GROUP + gi % gh;
+    tp = __builtin_amdgcn_readfirstlane(gi / gh);  // the compiler divides in vector registers
+    tq = __builtin_amdgcn_readfirstlane(grp * GROUP + gi % gh);
 }
 
 }  // namespace lin

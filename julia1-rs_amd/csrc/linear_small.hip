@@ -17,6 +17,54 @@ namespace {
 
 constexpr int NW = 8;
 
+// The residual of eight columns of one row, raw (e4m3 operands with FP32 outputs are E4m3Wide).
+template <class T>
+struct Resid8 {
+    static constexpr bool HALF_ONLY = __is_same(T, E4m3);
+    u32x4 v[HALF_ONLY ? 1 : 2];
+    __device__ void load(const LinearArgs& a, long t, int c0) {
+        const long at = min(t, (long)a.q_rows - 1) * a.ldr + min(c0, a.p_cols - 8);
+        if (!HALF_ONLY && a.out_f32) {
+            v[0] = *(const u32x4*)((const float*)a.resid + at);
+            v[HALF_ONLY ? 0 : 1] = *(const u32x4*)((const float*)a.resid + at + 4);
+        } else {
+            v[0] = *(const u32x4*)((const uint16_t*)a.resid + at);
+        }
+    }
+};
+
+// Eight columns of one output row from their sums z: c0 .. c0+7.
+template <class T>
+__device__ inline void finish8(const LinearArgs& a, float (&z)[8], long t, int c0, float qs, const ColumnTerms<T>& col,
+                               const Resid8<T>& resid) {
+    col.apply(a, z, qs);
+    if constexpr (T::bytes == 2)
+        if (a.pre) store16<T>((uint16_t*)a.pre + t * a.ldpre + c0, z);
+    activate(z, a.act);
+    if (!Resid8<T>::HALF_ONLY && a.out_f32) {
+        if (a.resid) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t r = resid.v[Resid8<T>::HALF_ONLY ? 0 : e >> 2][e & 3];
+                z[e] += __builtin_bit_cast(float, r);
+            }
+        }
+        float* o = (float*)a.out + t * a.ldo + c0;
+        *(f32x4*)o = f32x4{z[0], z[1], z[2], z[3]};
+        *(f32x4*)(o + 4) = f32x4{z[4], z[5], z[6], z[7]};
+    } else {
+        if (a.resid) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t r = resid.v[0][e];
+                z[2 * e] += T::lo(r);
+                z[2 * e + 1] += T::hi(r);
+            }
+        }
+        store16<T>((uint16_t*)a.out + t * a.ldo + c0, z);
+    }
+}
+
 template <class T, int EPI>
 __global__ __launch_bounds__(64 * NW) void linear_small_kernel(LinearArgs a) {
     constexpr int ES = T::bytes, PT = EPI == EPI_GATED ? 2 : 1;  // blocks of 16 P rows
