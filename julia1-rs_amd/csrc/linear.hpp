@@ -422,8 +422,8 @@ __device__ inline void finish_gated8(const LinearArgs& a, float (&g)[8], float (
 }
 
 // Epilogue of a wave's block of 64 P rows and 16 NJ output rows, the first of them t0; col0
-// is its first output column.  HALF: after that many blocks of 16 rows (and, where P is by
-// columns, after 32 columns) the rest lies 128 rows (columns) beyond the block's first.
+// is its first output column.  HALF: after that many blocks of 16 rows the rest lies 128 rows
+// beyond the block's first.
 // EARLY: what the epilogue reads is loaded by start(), under the multiplications; without it,
 // column terms by finish() and residuals four row blocks at a time, into the registers
 // that the fragments no longer need.
@@ -438,7 +438,7 @@ struct Epilogue {
 
     __device__ Epilogue(const LinearArgs& args, int row0, int col0, int lane_id) : a(args), t0(row0), lane(lane_id) {
         const int g = lane >> 4;
-        c0 = col0 + (HALF < NJ && LAYOUT != ROWS_ROWS ? (g & 1) * 16 + (g >> 1) * 128 : g * (EPI == EPI_GATED ? 8 : 16));
+        c0 = col0 + g * (EPI == EPI_GATED ? 8 : 16);
     }
     __device__ int first_row(int j) const { return t0 + (j < HALF ? j * 16 : 128 + (j - HALF) * 16); }
     __device__ int row(int j) const { return first_row(j) + (lane & 15); }
