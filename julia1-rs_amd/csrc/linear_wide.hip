@@ -26,12 +26,13 @@
 // The two waves of a SIMD (w and w + 4) run one half phase apart, waves 4-7 having met one
 // barrier more: while one multiplies, the other reads and issues.
 //
-// LDS holds two K steps of four 16 KB parts: the first and last 128 rows (columns, where k is the
-// row index: one run of 256 bytes per k; the weight gradient of 29367 x 3464 x 1504 took 403 us so,
-// 426 in runs of 64 and 128) of either operand, of which a wave reads 64 of P's and 32 of Q's.
-// Gated, P's first part is the gate's 128 rows and its second the up projection's.  So a lane ends
-// with 16 consecutive output columns, and four lanes with 64 of a row, whatever the layout: the
-// epilogue writes whole 128-byte lines.  A part read in
+// LDS holds two K steps of four 16 KB parts, two of either operand.  Q's hold its first and last
+// 128 rows (columns, where k is the row index), 32 of each for a wave.  P's: by columns the first
+// and last 128, 64 of each for a wave (one run of 256 bytes per k; the weight gradient of 29367 x
+// 3464 x 1504 took 403 us so, 426 in runs of 64 and 128); by rows the first and last 64 of a
+// wave's 128 (16384 x 4096 x 512: 91 us, 94 with the halves 128 apart); gated the gate's 128 rows
+// and the up projection's.  So a lane ends with 16 consecutive output columns and four lanes with
+// 64 of a row, whatever the layout: the epilogue writes whole 128-byte lines.  A part read in
 // one phase is refilled in the next: every wave has waited for its own reads (lgkmcnt) before
 // the barrier that the refilling waves have passed.  A part is read seven phases after its
 // issue, and one phase after every wave has waited for its own share of it: a wave issues two
@@ -109,7 +110,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     // halves of an operand: the second half lies p_half (q_half) bytes further.
     const uint8_t* const pb = (const uint8_t*)a.p + (P_COLS ? (long)p0 : (long)p0 * a.ldp) * ES;
     const uint8_t* const qb = (const uint8_t*)a.q + (Q_COLS ? (long)q0 : (long)q0 * a.ldq) * ES;
-    const long p_half = P_COLS ? 128 * ES : (EPI == EPI_GATED ? (long)a.p_cols : 128L) * a.ldp * ES;
+    const long p_half = P_COLS ? 128 * ES : (EPI == EPI_GATED ? (long)a.p_cols : 64L) * a.ldp * ES;
     const long q_half = (Q_COLS ? 128L : 128 * a.ldq) * ES;
     const int p_rows = EPI == EPI_GATED ? 2 * a.p_cols - p0 : a.p_cols - p0;
     const long p_bytes = ((long)(p_rows - 1) * a.ldp + a.k) * ES, q_bytes = ((long)(a.q_rows - q0 - 1) * a.ldq + a.k) * ES;
@@ -130,7 +131,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         const uint32_t rk = ((lane & 7) ^ row_swz(r)) * 16;
         tail[j] = __builtin_amdgcn_ballot_w64((steps - 1) * STEP_BYTES + rk < kbytes);
         poff[j] = P_COLS ? (uint32_t)((k * a.ldp + q * 8) * ES)
-                         : (uint32_t)(p_row<EPI_LINEAR>(r, 0) * a.ldp * ES + rk);
+                         : (uint32_t)((p_row<EPI_LINEAR>(r, 0) + (EPI == EPI_GATED ? 0 : r & 64)) * a.ldp * ES + rk);
         qoff[j] = Q_COLS ? (uint32_t)((k * a.ldq + q * 8) * ES) : (uint32_t)(r * a.ldq * ES + rk);
     }
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)&smem[wave * 2048]);
@@ -226,15 +227,16 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     // No load may still be on its way into LDS when the workgroup ends.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
-    // The second half of the wave's Q rows lies 128 rows on, and so do its P columns.
-    const int col0 = p0 + wp * 64, t0 = q0 + wq * 32;
+    // The second half of the wave's Q rows lies 128 rows on.
+    const int t0 = q0 + wq * 32;
     const int l = (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0));  // `lane`, not kept over the loop
     if constexpr (EPI == EPI_GATED) {
-        finish_gated<T>(a, acc, t0, col0 + (l >> 4) * 16, l);
+        finish_gated<T>(a, acc, t0, p0 + wp * 64 + (l >> 4) * 16, l);
     } else {
-        Epilogue<T, LAYOUT, EPI, 4, 2, false>(a, t0, col0, l).finish(acc[0], split);
+        const int first = p0 + wp * (P_COLS ? 64 : 128), second = first + (P_COLS ? 128 : 64);
+        Epilogue<T, LAYOUT, EPI, 4, 2, false>(a, t0, first, l).finish(acc[0], split);
         __builtin_amdgcn_sched_barrier(0);
-        Epilogue<T, LAYOUT, EPI, 4, 2, false>(a, t0, col0 + 128, l).finish(acc[1], split);
+        Epilogue<T, LAYOUT, EPI, 4, 2, false>(a, t0, second, l).finish(acc[1], split);
     }
 }
 
