@@ -49,7 +49,7 @@ __device__ inline void load8_of(const void* p, float (&v)[8]) {
 // dz = dy act'(pre) (rounded to T) and the column sums of its unrounded values, a part per
 // blockIdx.y.  A lane owns 8 columns, the four waves of a workgroup every fourth of its rows;
 // their sums are joined in wave order.  dz is kept because both products read it, one of them by
-// columns.  Bound by memory: 9482 x 1024 bf16 gelu, 58 MB, takes 18 us (3.2 TB/s; 21 with four rows
+// columns.  Bound by memory: 9482 x 1024 bf16 gelu, 58 MB, takes 18 to 20 us (3.1 TB/s; 3 more with four rows
 // in flight per wave).
 template <class T>
 __global__ __launch_bounds__(THREADS) void act_grad_kernel(ActGradArgs a) {
@@ -278,15 +278,16 @@ LinearArgs row_range(const LinearArgs& a, int r0, int rows) {
 
 // Rows that 256 x 256 tiles take in whole rounds of the CUs, where that and another kernel
 // for the rest come cheaper than any kernel alone; else 0.  18000 x 1024 x 4096 (284 tiles): 164
-// us at once, 127 as 16384 rows and 1616 on 64 x 64 tiles; 5000 x 4096 x 4096: 161 and 138; with a
-// last round half full it is even (9482 x 2304 x 768: 46.5 and 47.4).
+// us at once, 127 as 16384 rows and 1616 on 64 x 64 tiles; 5000 x 4096 x 4096: 161 and 138.  The
+// second launch and the drain between cost 3 us, so that a last round half full stays where it is
+// (9482 x 2304 x 768: 46.5 us, in two 48.4).
 int whole_rounds(const LinearArgs& a, double alone) {
     if (a.type == JH_E4M3 && a.out_f32) return 0;
     const long across = tiles_of(row_range(a, 0, 1), 256, 256), rounds = tiles_of(a, 256, 256) / CUS;
     const long rows = rounds * CUS / across * 256;
     if (rows <= 0 || rows >= a.q_rows) return 0;
     const double c = cost(WIDE, row_range(a, 0, (int)rows), 1) +
-                     pick(row_range(a, (int)rows, a.q_rows - (int)rows), false).cost;
+                     pick(row_range(a, (int)rows, a.q_rows - (int)rows), false).cost + 3.0;
     return c < alone ? (int)rows : 0;
 }
 

@@ -2,13 +2,13 @@
 // workgroup per CU.  Against 128 x 128 tiles this halves the operand bytes that L2 and the
 // LDS DMA move per MFMA.
 //
-// Measured (MFMA busy and clock from counters): 16384 x 8192 x 2048 bf16 gated with silu, 1.10
-// PFLOP in 917 us (1.20 PFLOP/s, busy 59 % at 1.93 GHz: power holds the clock there, 2.4 GHz at
-// rest); 8192^3 bf16 0.92 ms (1.19 PFLOP/s; by columns 1.29 for dx, 1.19 for dw); 4096^3 e4m3 57 us
-// (2.40 PFLOP/s); 8192 x 4096 x 4096 e4m3 with bias, silu and residual 127 us (2.17), whose tiles
-// end together twice: 67 MB of residuals and outputs in a burst, 13 of 63 us at the memory's rate.
-// LDS is read a fifth of the time, without bank conflicts; a step's 64 KB of operands take half as
-// long to come in as its MFMAs (2048 cycles), all CUs reading.
+// Measured (MFMA busy and clock from counters): 16384 x 8192 x 2048 bf16 gated with silu and both
+// projections kept, 1.10 PFLOP in 891 us (1.23 PFLOP/s, busy 59 % at 1.91 GHz: power holds the
+// clock there, 2.4 GHz at rest); 8192 x 4096 x 4096 bf16 200 us (1.37); 4096^3 e4m3 57 us (2.40);
+// 8192 x 4096 x 4096 e4m3 105 us (2.6), with bias, silu and residual 125 (2.2): all tiles of a
+// round end together, 67 MB of residuals and outputs in a burst, twice.  LDS is read a fifth of
+// the time, without bank conflicts; a step's 64 KB of operands take half as long to come in as its
+// MFMAs (2048 cycles), all CUs reading.
 //
 // A K step runs in four phases, each a quadrant of the wave's block: 64 P rows by 32 Q rows,
 // 16 MFMAs of 16 bits.  A phase first reads the fragments that it or the next lacks and
