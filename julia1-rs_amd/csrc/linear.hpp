@@ -187,6 +187,8 @@ __device__ inline void dma16(uint32_t lds, uint32_t voff, i32x4 rsrc, uint32_t s
 // The fragment of 16 columns and K half h is k = 32h + 8g + (0..7), by two transposing reads
 // (in each 16 lanes, lane j addresses row j / 4 and columns 4 (j % 4); lane i receives four
 // rows of column i).  TILES: the 16-column tiles that the wave reads of a part.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Wint-to-pointer-cast"  // LDS addresses have 32 bits, which the host pass does not know
 template <class T, bool COLS, int TILES, int WIDTH = 128>
 struct FragReader {
     static constexpr int N = COLS ? TILES : 1;
@@ -232,6 +234,7 @@ struct FragReader {
         }
     }
 };
+#pragma clang diagnostic pop
 
 // ---------------------------------------------------------------- epilogue
 
