@@ -26,20 +26,12 @@ E4M3_MAX = 448.0
 EPS = 1e-6
 
 
-_loaded = None
-
-
 def _hip():
-    """The framework's operators, imported once, as a user's program does."""
-    global _loaded
-    if _loaded is not None:
-        return _loaded
     path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "julia1-rs_amd")
     if path not in sys.path:
         sys.path.insert(0, path)
     from julia1_amd import hip
 
-    _loaded = hip
     return hip
 
 
