@@ -357,6 +357,30 @@ int jh_op_gated_ffn_backward(int type, const void* dh, size_t lddh, const void* 
                              void* stream);
 size_t jh_op_gated_ffn_backward_workspace(size_t rows, size_t inter, size_t k);
 
+/*
+ * Which kernels a product runs on, as the calls above choose them by size: jh_op_linear's
+ * (LINEAR; n, k as there), jh_op_gated_ffn's (GATED; n its inter) and the gradients' dx and dw (DX, DW;
+ * n and k as in jh_op_linear_backward, n = 2 inter for the gated projections').  Two launches
+ * where the first takes whole rounds of 256 x 256 tiles and the second the other rows, else
+ * launches[1].rows is 0.  rows counts the output's (DW: n of them in all), parts the pieces
+ * of the contraction that are summed by one more kernel.  Needs no device.
+ */
+enum { JH_PRODUCT_LINEAR = 0, JH_PRODUCT_GATED = 1, JH_PRODUCT_DX = 2, JH_PRODUCT_DW = 3 };
+enum {
+    JH_KERNEL_SMALL = 0,   /* 64 x 64 tiles                                           */
+    JH_KERNEL_GROUP = 1,   /* 64 x 64, four groups of waves share the contraction     */
+    JH_KERNEL_DEEP = 2,    /* 128 x 128, one tile to a CU                             */
+    JH_KERNEL_PAIR = 3,    /* 128 x 128, two to a CU                                  */
+    JH_KERNEL_TALL = 4,    /* 256 rows x 128 columns                                  */
+    JH_KERNEL_WIDE = 5,    /* 256 x 256                                               */
+    JH_KERNEL_STREAM = 6   /* up to 16 rows, w streams past them                      */
+};
+typedef struct {
+    int kernel, parts;
+    size_t rows;
+} jh_linear_launch;
+int jh_op_linear_plan(int product, int type, int out_type, size_t rows, size_t n, size_t k, jh_linear_launch launches[2]);
+
 #ifdef __cplusplus
 }
 #endif

@@ -243,6 +243,13 @@ struct RmsNormGradArgs {
 void linear_forward(const LinearArgs& a, size_t rows, size_t n, size_t k, int out_type, hipStream_t stream);
 void linear_backward(const LinearGradArgs& a, size_t rows, size_t n, size_t k, hipStream_t stream);
 size_t linear_backward_workspace(size_t rows, size_t n, size_t k, int act, bool gated);
+// The one or two launches of a product (a second of 0 rows: none); see jh_op_linear_plan.
+struct LinearPlan {
+    struct {
+        int kernel, parts, rows;
+    } launch[2];
+};
+LinearPlan linear_plan(int product, int type, int out_type, size_t rows, size_t n, size_t k);
 
 // One kernel each: 256 x 256 tiles, smaller tiles, and few rows.
 void launch_linear_wide(const LinearArgs& a, hipStream_t stream);  // not e4m3 operands with an FP32 output

@@ -184,7 +184,8 @@ long tiles_of(const LinearArgs& a, int p, int q) {
 //   dx of 9482 x 2304 x 768   70.1    91.0    48.2    [37.4]          50.0
 //   dw of 4096 x 4096 x 1024  66.1    78.7    [40.0]  50.2            98.2
 //   dw of 8192 x 4096 x 4096  527     742     340     264             [223]
-enum { SMALL, GROUP, DEEP, PAIR, TALL, WIDE, KERNELS };
+enum { SMALL = JH_KERNEL_SMALL, GROUP = JH_KERNEL_GROUP, DEEP = JH_KERNEL_DEEP, PAIR = JH_KERNEL_PAIR, TALL = JH_KERNEL_TALL,
+       WIDE = JH_KERNEL_WIDE, KERNELS };
 constexpr long CUS = 256;
 
 double cost(int kernel, const LinearArgs& a, long splits) {
@@ -231,8 +232,16 @@ double cost(int kernel, const LinearArgs& a, long splits) {
     }
 }
 
+// Whether a launch can hold the kernel's tiles along x, where it has fewer than 2^32 threads.  (2^30 rows
+// by 8 columns: 2^24 tiles of 64 x 64 by 256 threads are too many, 2^23 of 128 x 128 are not.)
+bool launches(int kernel, const LinearArgs& a) {
+    const int side = kernel == WIDE ? 256 : kernel == SMALL || kernel == GROUP ? 64 : 128;
+    const long threads = kernel == GROUP ? 1024 : kernel == SMALL || kernel == PAIR ? 256 : 512;
+    return tiles_of(a, side, kernel == TALL ? 256 : side) * threads < 1L << 32;
+}
+
 struct Choice {
-    int kernel;
+    int kernel;  // KERNELS: none can be launched
     int splits;
     double cost;
 };
@@ -243,7 +252,7 @@ struct Choice {
 constexpr long MAX_SPLITS = 16, MIN_STEPS = 4;
 long split_bytes(const LinearArgs& a) { return (a.layout == COLS_COLS ? 192L : 48L) << 20; }
 Choice pick(const LinearArgs& a, bool gradient) {
-    Choice best{PAIR, 1, 1e30};
+    Choice best{KERNELS, 1, 1e30};
     const double out = (double)a.q_rows * a.p_cols * 4;
     for (long splits = 1; splits <= (gradient ? MAX_SPLITS : 1); splits += splits < 4 ? 1 : splits < 8 ? 2 : 4) {
         if (splits > 1 && (steps_of(a) < splits * MIN_STEPS || out * splits > split_bytes(a))) break;
@@ -256,6 +265,7 @@ Choice pick(const LinearArgs& a, bool gradient) {
             // The groups share a long contraction; k contiguous that gains only where both operands are
             // in L2 already (128 x 1024 x 4096: 15.1 us against Small's 17.5, else 20.0 against 17.7)
             if (kernel == GROUP && a.layout == ROWS_ROWS) continue;
+            if (!launches(kernel, a)) continue;
             const double c = cost(kernel, a, splits) + sum;
             if (c < best.cost) best = {kernel, (int)splits, c};
         }
@@ -285,19 +295,41 @@ int whole_rounds(const LinearArgs& a, double alone) {
     if (a.type == JH_E4M3 && a.out_f32) return 0;
     const long across = tiles_of(row_range(a, 0, 1), 256, 256), rounds = tiles_of(a, 256, 256) / CUS;
     const long rows = rounds * CUS / across * 256;
-    if (rows <= 0 || rows >= a.q_rows) return 0;
+    if (rows <= 0 || rows >= a.q_rows || !launches(WIDE, row_range(a, 0, (int)rows))) return 0;
     const double c = cost(WIDE, row_range(a, 0, (int)rows), 1) +
                      pick(row_range(a, (int)rows, a.q_rows - (int)rows), false).cost + 3.0;
     return c < alone ? (int)rows : 0;
 }
 
-long partial_bytes(const LinearArgs& a) {
-    const int s = pick(a, true).splits;
-    return s > 1 ? round_up((long)s * a.q_rows * a.p_cols * 4, 256) : 0;
+// What a product runs on, settled before anything is launched: one kernel, or 256 x 256 tiles for its
+// first `whole` rows and another kernel for the rest.
+struct Plan {
+    int kernel, splits, whole, rest;
+};
+
+// Up to 16 rows, W streams past them from memory (16 x 4096 x 4096: 10.1 us, 16.5 on 64 x 64
+// tiles; 17 to 32 rows, two blocks of them, took 18.2 against 17.6).
+constexpr int STREAM_ROWS = 16;
+
+Plan plan(const char* op, const LinearArgs& a, bool gradient) {
+    if (!gradient && a.q_rows <= STREAM_ROWS) return {JH_KERNEL_STREAM, 1, 0, 0};
+    const Choice c = pick(a, gradient);
+    if (c.kernel == KERNELS) throw jh_error(JH_ERR_INVALID, std::string(op) + ": too large");
+    Plan p{c.kernel, c.splits, c.splits == 1 ? whole_rounds(a, c.cost) : 0, 0};
+    if (p.whole) {
+        p.kernel = WIDE;
+        p.rest = pick(row_range(a, p.whole, a.q_rows - p.whole), false).kernel;
+    }
+    return p;
+}
+
+long partial_bytes(const LinearArgs& a, const Plan& p) {
+    return p.splits > 1 ? round_up((long)p.splits * a.q_rows * a.p_cols * 4, 256) : 0;
 }
 
 void launch(int kernel, const LinearArgs& a, hipStream_t s) {
-    if (kernel == WIDE) launch_linear_wide(a, s);
+    if (kernel == JH_KERNEL_STREAM) launch_linear_small(a, s);
+    else if (kernel == WIDE) launch_linear_wide(a, s);
     else launch_linear_tile(a, kernel == SMALL ? LinearTile::Small : kernel == GROUP ? LinearTile::Group
                                : kernel == DEEP ? LinearTile::Deep : kernel == PAIR ? LinearTile::Pair : LinearTile::Tall, s);
 }
@@ -310,36 +342,17 @@ void split_sum(const LinearArgs& a, hipStream_t s) {
     HIP_CHECK(hipGetLastError());
 }
 
-// Up to 16 rows, W streams past them from memory (16 x 4096 x 4096: 10.1 us, 16.5 on 64 x 64
-// tiles; 17 to 32 rows, two blocks of them, took 18.2 against 17.6).
-constexpr int STREAM_ROWS = 16;
-
-void run_whole(const LinearArgs& a, const Choice& c, hipStream_t s) {
-    if (const int rows = whole_rounds(a, c.cost)) {
-        const LinearArgs rest = row_range(a, rows, a.q_rows - rows);
-        launch(WIDE, row_range(a, 0, rows), s);
-        launch(pick(rest, false).kernel, rest, s);
-    } else {
-        launch(c.kernel, a, s);
+// A product by its plan; the parts of a contraction that is split go to `partial`.
+void run(LinearArgs a, const Plan& p, float* partial, hipStream_t s) {
+    a.splits = p.splits;
+    a.split_steps = p.splits > 1 ? (int)((steps_of(a) + p.splits - 1) / p.splits) : 0x7fffffff;
+    a.partial = p.splits > 1 ? partial : nullptr;
+    if (p.whole) {
+        launch(p.kernel, row_range(a, 0, p.whole), s);
+        return launch(p.rest, row_range(a, p.whole, a.q_rows - p.whole), s);
     }
-}
-
-void run(LinearArgs a, hipStream_t s) {
-    a.splits = 1;
-    a.split_steps = 0x7fffffff;
-    if (a.q_rows <= STREAM_ROWS) launch_linear_small(a, s);
-    else run_whole(a, pick(a, false), s);
-}
-
-// A gradient product, its contraction split where that fills the GPU.
-void run_gradient(LinearArgs a, float* partial, hipStream_t s) {
-    if (a.q_rows == 0) return;
-    const Choice c = pick(a, true);
-    a.split_steps = (int)((steps_of(a) + c.splits - 1) / c.splits);
-    a.splits = c.splits;
-    a.partial = c.splits > 1 ? partial : nullptr;
-    if (c.splits == 1) return run_whole(a, c, s);
-    launch(c.kernel, a, s);
+    launch(p.kernel, a, s);
+    if (p.splits == 1) return;
     if (a.type == JH_BF16) split_sum<Bf16>(a, s);
     else split_sum<F16>(a, s);
 }
@@ -449,7 +462,28 @@ void linear_forward(const LinearArgs& args, size_t rows, size_t n, size_t k, int
     }
     // out may be resid itself: every element is read by the thread that writes it.
     if (a.resid != a.out || a.ldr != a.ldo) check_disjoint(op, "out", out, "resid", resid);
-    run(a, s);
+    run(a, plan(op, a, false), nullptr, s);
+}
+
+LinearPlan linear_plan(int product, int type, int out_type, size_t rows, size_t n, size_t k) {
+    const char* op = "linear_plan";
+    if (product < JH_PRODUCT_LINEAR || product > JH_PRODUCT_DW) refuse(op, "unknown product");
+    check_sizes(op, type, rows, n, k);
+    const bool gradient = product >= JH_PRODUCT_DX;
+    const int half = type == JH_E4M3 ? JH_BF16 : type;
+    if (gradient && type == JH_E4M3) refuse(op, "gradients are of bf16 or f16 operands");
+    if (out_type != half && (out_type != JH_F32 || product == JH_PRODUCT_GATED || product == JH_PRODUCT_DX))
+        refuse(op, "no such output type");
+    LinearArgs a{};
+    a.type = type;
+    a.gated = product == JH_PRODUCT_GATED;
+    a.out_f32 = out_type == JH_F32;
+    a.layout = product == JH_PRODUCT_DX ? COLS_ROWS : product == JH_PRODUCT_DW ? COLS_COLS : ROWS_ROWS;
+    a.q_rows = (int)(product == JH_PRODUCT_DW ? n : rows);
+    a.p_cols = (int)(gradient ? k : n);
+    a.k = (int)(product == JH_PRODUCT_DW ? rows : product == JH_PRODUCT_DX ? n : k);
+    const Plan p = plan(op, a, gradient);
+    return {{{p.kernel, p.splits, p.whole ? p.whole : a.q_rows}, {p.rest, p.whole ? 1 : 0, p.whole ? a.q_rows - p.whole : 0}}};
 }
 
 namespace {
@@ -458,12 +492,13 @@ namespace {
 // column sums, and after them of the products: the stream runs one after the other).
 struct BackwardPlan {
     LinearArgs dx{}, dw{};
+    Plan dx_plan{}, dw_plan{};
     long dz_bytes = 0, part_bytes = 0;
     int sum_blocks = 0, rows_per_block = 0;
     size_t bytes() const { return (size_t)(dz_bytes + part_bytes); }
 };
 
-BackwardPlan plan_backward(int type, size_t rows, size_t n, size_t k, bool keeps_dz, bool sums) {
+BackwardPlan plan_backward(const char* op, int type, size_t rows, size_t n, size_t k, bool keeps_dz, bool sums) {
     BackwardPlan p;
     p.dx.type = p.dw.type = type;
     p.dx.layout = COLS_ROWS;
@@ -474,14 +509,14 @@ BackwardPlan plan_backward(int type, size_t rows, size_t n, size_t k, bool keeps
     p.dw.p_cols = (int)k;
     p.dw.q_rows = (int)n;
     p.dw.k = (int)rows;
+    p.dx_plan = plan(op, p.dx, true);
+    p.dw_plan = plan(op, p.dw, true);
     p.dz_bytes = keeps_dz ? round_up((long)rows * n * 2, 256) : 0;
-    p.part_bytes = std::max(partial_bytes(p.dx), partial_bytes(p.dw));
-    if (sums) {
-        const long across = (n + 511) / 512, want = std::max(1L, 1024 / across);
-        p.rows_per_block = (int)std::max(8L, ((long)rows + want - 1) / want);
-        p.sum_blocks = (int)(((long)rows + p.rows_per_block - 1) / p.rows_per_block);
-        p.part_bytes = std::max(p.part_bytes, round_up((long)p.sum_blocks * n * 4, 256));
-    }
+    p.part_bytes = std::max(partial_bytes(p.dx, p.dx_plan), partial_bytes(p.dw, p.dw_plan));
+    const long across = (n + 511) / 512, want = std::max(1L, 1024 / across);
+    p.rows_per_block = (int)std::max(8L, ((long)rows + want - 1) / want);
+    p.sum_blocks = (int)(((long)rows + p.rows_per_block - 1) / p.rows_per_block);
+    if (sums) p.part_bytes = std::max(p.part_bytes, round_up((long)p.sum_blocks * n * 4, 256));
     return p;
 }
 
@@ -494,7 +529,7 @@ void check_workspace(const char* op, const void* ws, size_t bytes, size_t need) 
 // The two gradient products of a linear layer: dx = dz W and dw = dzᵀ x.
 void run_products(const BackwardPlan& p, const void* dz, long lddz, const LinearGradArgs& a, float* partial,
                   hipStream_t s) {
-    if (a.dx) {
+    if (a.dx && p.dx.q_rows) {
         LinearArgs d = p.dx;
         d.p = a.w;
         d.ldp = p.dx.p_cols;
@@ -502,7 +537,7 @@ void run_products(const BackwardPlan& p, const void* dz, long lddz, const Linear
         d.ldq = lddz;
         d.out = a.dx;
         d.ldo = a.lddx;
-        run_gradient(d, partial, s);
+        run(d, p.dx_plan, partial, s);
     }
     if (a.dw) {
         LinearArgs d = p.dw;
@@ -513,7 +548,7 @@ void run_products(const BackwardPlan& p, const void* dz, long lddz, const Linear
         d.out = a.dw;
         d.ldo = p.dw.p_cols;
         d.out_f32 = a.grad_f32;
-        run_gradient(d, partial, s);
+        run(d, p.dw_plan, partial, s);
     }
 }
 
@@ -524,7 +559,7 @@ size_t linear_backward_workspace(size_t rows, size_t n, size_t k, int act, bool 
     check_sizes(op, JH_BF16, rows, n, k);
     if (gated && n % 16) refuse(op, "output features must be a multiple of 8");
     check_act(op, act);
-    return plan_backward(JH_BF16, rows, n, k, gated || act != JH_ACT_NONE, !gated).bytes();
+    return plan_backward(op, JH_BF16, rows, n, k, gated || act != JH_ACT_NONE, !gated).bytes();
 }
 
 void linear_backward(const LinearGradArgs& args, size_t rows, size_t n, size_t k, hipStream_t s) {
@@ -542,7 +577,7 @@ void linear_backward(const LinearGradArgs& args, size_t rows, size_t n, size_t k
     a.ldpre = row_stride(a.ldpre, rows, n);
     a.ldx = row_stride(a.ldx, rows, k);
     a.lddx = row_stride(a.lddx, rows, k);
-    const BackwardPlan p = plan_backward(a.type, rows, n, k, keeps_dz, a.dbias != nullptr);
+    const BackwardPlan p = plan_backward(op, a.type, rows, n, k, keeps_dz, a.dbias != nullptr);
     check_workspace(op, a.workspace, a.workspace_bytes, p.bytes());
     const Span ws = span_of(a.workspace, p.bytes(), p.bytes() ? 1 : 0, p.bytes(), JH_E4M3);
     if (rows) check_matrix(op, a.gated ? "dh" : "dy", a.dy, a.lddy, rows, dy_cols, a.type);
@@ -581,17 +616,15 @@ void linear_backward(const LinearGradArgs& args, size_t rows, size_t n, size_t k
         else JH_LAUNCH(gated_grad_kernel<F16>, grid, dim3(THREADS), 0, s, g);
         HIP_CHECK(hipGetLastError());
     } else if (!a.gated && (keeps_dz || a.dbias)) {
-        // Rows per workgroup are the plan's with the sums, as the parts are stored by them.
-        const BackwardPlan q = plan_backward(a.type, rows, n, k, keeps_dz, true);
         if (rows) {
             const ActGradArgs g{a.dy, a.lddy, keeps_dz ? a.pre : nullptr, a.ldpre, base, a.dbias ? partial : nullptr,
-                                (int)rows, (int)n, q.rows_per_block, a.act};
-            const dim3 grid((unsigned)((n + 511) / 512), (unsigned)q.sum_blocks);
+                                (int)rows, (int)n, p.rows_per_block, a.act};
+            const dim3 grid((unsigned)((n + 511) / 512), (unsigned)p.sum_blocks);
             if (a.type == JH_BF16) JH_LAUNCH(act_grad_kernel<Bf16>, grid, dim3(THREADS), 0, s, g);
             else JH_LAUNCH(act_grad_kernel<F16>, grid, dim3(THREADS), 0, s, g);
             HIP_CHECK(hipGetLastError());
         }
-        if (a.dbias) launch_column_sum(partial, q.sum_blocks, (int)n, a.dbias, s);
+        if (a.dbias) launch_column_sum(partial, p.sum_blocks, (int)n, a.dbias, s);
     }
     run_products(p, dz, lddz, a, partial, s);
 }

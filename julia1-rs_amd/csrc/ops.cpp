@@ -228,6 +228,14 @@ size_t jh_op_linear_backward_workspace(size_t rows, size_t n, size_t k, int act)
     return bytes;
 }
 
+int jh_op_linear_plan(int product, int type, int out_type, size_t rows, size_t n, size_t k, jh_linear_launch launches[2]) {
+    return jh_guarded([&] {
+        if (!launches) throw jh_error(JH_ERR_INVALID, "linear_plan: launches is null");
+        const LinearPlan p = linear_plan(product, type, out_type, rows, n, k);
+        for (int i = 0; i < 2; ++i) launches[i] = {p.launch[i].kernel, p.launch[i].parts, (size_t)p.launch[i].rows};
+    });
+}
+
 int jh_op_gated_ffn(int type, const void* x, size_t ldx, const float* x_scale, size_t rows, const void* wi,
                     const float* wi_scale, size_t inter, size_t k, int act, void* out, size_t ldo, void* gu,
                     size_t ldgu, void* stream) {

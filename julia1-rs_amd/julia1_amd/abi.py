@@ -35,6 +35,9 @@ EPI_BIAS_F32 = 6
 # element types and activations of jh_op_rms_norm, jh_op_linear and jh_op_gated_ffn
 F32, BF16, F16, E4M3 = range(4)
 ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = range(5)
+# products and kernels of jh_op_linear_plan
+PRODUCT_LINEAR, PRODUCT_GATED, PRODUCT_DX, PRODUCT_DW = range(4)
+KERNEL_SMALL, KERNEL_GROUP, KERNEL_DEEP, KERNEL_PAIR, KERNEL_TALL, KERNEL_WIDE, KERNEL_STREAM = range(7)
 
 _f32p = C.POINTER(C.c_float)
 

@@ -25,7 +25,7 @@ EXPORTS = (
     "jh_op_embed_ln", "jh_op_layer_norm", "jh_op_final_norm",
     "jh_op_gather_f32", "jh_op_scorer", "jh_op_attention", "jh_op_attention_wide", "jh_op_attention_unsplit",
     "jh_op_rms_norm", "jh_op_rms_norm_backward", "jh_op_rms_norm_backward_workspace", "jh_op_quantize_rows",
-    "jh_op_linear", "jh_op_linear_backward", "jh_op_linear_backward_workspace",
+    "jh_op_linear", "jh_op_linear_backward", "jh_op_linear_backward_workspace", "jh_op_linear_plan",
     "jh_op_gated_ffn", "jh_op_gated_ffn_backward", "jh_op_gated_ffn_backward_workspace",
 )
 
@@ -33,6 +33,10 @@ EXPORTS = (
 class KernelStat(C.Structure):
     _fields_ = [("name", C.c_char_p), ("launches", C.c_uint32), ("ms", C.c_double), ("flops", C.c_double),
                 ("bytes", C.c_double)]
+
+
+class LinearLaunch(C.Structure):
+    _fields_ = [("kernel", C.c_int), ("parts", C.c_int), ("rows", C.c_size_t)]
 
 
 class HipError(RuntimeError):
@@ -104,6 +108,7 @@ def lib():
         L.jh_op_gated_ffn.argtypes = [i32, vp, sz, vp, sz, vp, vp, sz, sz, i32, vp, sz, vp, sz, vp]
         L.jh_op_gated_ffn_backward.argtypes = [i32, vp, sz, vp, sz, vp, sz, sz, vp, sz, sz, i32, vp, sz, i32, vp, vp,
                                                sz, vp]
+        L.jh_op_linear_plan.argtypes = [i32, i32, i32, sz, sz, sz, C.POINTER(LinearLaunch)]
         L.jh_op_rms_norm_backward_workspace.argtypes = [sz, sz]
         L.jh_op_linear_backward_workspace.argtypes = [sz, sz, sz, i32]
         L.jh_op_gated_ffn_backward_workspace.argtypes = [sz, sz, sz]
@@ -357,14 +362,19 @@ def _invalid(msg):
     raise HipError(abi.JH_ERR_INVALID, msg)
 
 
+def _dtype_codes():
+    if not _TYPES:
+        import torch
+        _TYPES.update({torch.float32: abi.F32, torch.bfloat16: abi.BF16, torch.float16: abi.F16,
+                       torch.float8_e4m3fn: abi.E4M3})
+    return _TYPES
+
+
 def _type(t):
     """The element type code of a torch tensor."""
     code = _TYPES.get(t.dtype)
     if code is None:
-        import torch
-        _TYPES.update({torch.float32: abi.F32, torch.bfloat16: abi.BF16, torch.float16: abi.F16,
-                       torch.float8_e4m3fn: abi.E4M3})
-        code = _TYPES.get(t.dtype)
+        code = _dtype_codes().get(t.dtype)
         if code is None:
             _invalid(f"no such element type: {t.dtype}")
     return code
@@ -535,6 +545,18 @@ def op_linear_backward(dy, x, w, workspace, act="none", pre=None, dx=None, dw=No
 
 def linear_backward_workspace(rows, n, k, act="none") -> int:
     return _bytes(lib().jh_op_linear_backward_workspace(rows, n, k, _act(act)))
+
+
+def linear_plan(product, dtype, rows, n, k, out_dtype=None):
+    """jh_op_linear_plan: [(kernel, parts, rows)] of the one or two launches of a product ("linear", "gated", "dx" or
+    "dw") of torch types; out_dtype is dtype (bfloat16 for e4m3) unless given."""
+    codes = _dtype_codes()
+    t = codes[dtype]
+    out = codes[out_dtype] if out_dtype is not None else abi.BF16 if t == abi.E4M3 else t
+    launches = (LinearLaunch * 2)()
+    check(lib().jh_op_linear_plan(("linear", "gated", "dx", "dw").index(product), t, out, rows, n, k, launches))
+    names = ("small", "group", "deep", "pair", "tall", "wide", "stream")
+    return [(names[v.kernel], v.parts, v.rows) for v in launches if v.parts]
 
 
 def op_gated_ffn(x, wi, out, act="gelu", x_scale=None, w_scale=None, gu=None, stream=None):
