@@ -259,7 +259,9 @@ enum {
  * can be captured into graphs.  A workspace is scratch of one call at a time: calls
  * that may run at once, replays of graphs among them, have one each.  Sums,
  * statistics and activations are FP32, results are rounded once, and every sum
- * has a fixed order: the same call gives the same bits.  A row's bits may depend
+ * has a fixed order: the same call gives the same bits.  GELU and SiLU are good to
+ * (8 + E) 2^-23 of their value, E = z^2 and |z| (the tanh form: 4 times the argument
+ * of its exponential), down to 2^-119.  A row's bits may depend
  * on the number of rows in the call (kernels are chosen by size).  Squares are
  * summed as they are: rows whose sum of squares passes 3.4e38 are not normalised.
  */

@@ -23,10 +23,10 @@ __device__ inline void act_and_grad(float z, int act, float& value, float& grad)
         grad = z > 0.0f ? 1.0f : 0.0f;
         if (z != z) grad = z;
     } else if (act == JH_ACT_GELU) {
-        const float cdf = 0.5f * (1.0f + erf_rational(z * 0.70710678118654752f));
-        const float pdf = 0.3989422804014327f * __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z);
-        value = z * cdf;
-        grad = __builtin_fmaf(z, pdf, cdf);
+        float a, e;
+        const float q = normal_tail(z, a, e), pdf = 0.3989422804014327f * e;
+        value = gelu_of(z, a, q);
+        grad = __builtin_fmaf(z, pdf, z < 0.0f ? q : 1.0f - q);
     } else {
         const float a = act == JH_ACT_SILU ? 1.0f : kTanhA, b = act == JH_ACT_SILU ? 0.0f : kTanhA * kTanhB;
         // z^2 short of infinity, whose products with 0 (b, or 1 - s) would be NaN

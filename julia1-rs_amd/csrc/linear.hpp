@@ -121,6 +121,29 @@ __device__ inline float sigmoid(float x) {
 constexpr float kTanhA = 1.5957691216057308f;   // 2 sqrt(2 / pi): gelu_tanh(z) = z sigmoid(A (z + B z^3))
 constexpr float kTanhB = 0.044715f;
 
+// The normal distribution's cdf at -|z|, good to (6 + z^2) 2^-23 of its value, with e = exp(-z^2 / 2)
+// (both 0 from |z| = 13.3 on) and a = |z| up to there.  cdf(-a) e^{a^2/2} is a quotient of polynomials
+// of degree 3 and 4: a least-squares fit over [0, 13.3], weighted until the largest relative
+// error was least, off by 3.6e-7.  1 + erf(z / sqrt 2) has the cdf's absolute precision only (gelu(-5)
+// was off by 6 % so), for as many instructions.
+__device__ inline float normal_tail(float z, float& a, float& e) {
+    a = fminf(__builtin_fabsf(z), 15.0f);
+    float n = 0.01686366f, d = 0.04227636f;
+    n = __builtin_fmaf(n, a, 0.11875391f);
+    d = __builtin_fmaf(d, a, 0.29745701f);
+    n = __builtin_fmaf(n, a, 0.36061483f);
+    d = __builtin_fmaf(d, a, 0.94971181f);
+    n = __builtin_fmaf(n, a, 0.49999982f);
+    d = __builtin_fmaf(d, a, 1.51909666f);
+    d = __builtin_fmaf(d, a, 1.0f);
+    e = __builtin_amdgcn_exp2f(-0.72134752044448170f * (a * a));
+    return n * __builtin_amdgcn_rcpf(d) * e;
+}
+// z cdf(z) = max(z, 0) - |z| cdf(-|z|); a NaN stays one.
+__device__ inline float gelu_of(float z, float a, float q) {
+    return __builtin_fmaf(-a, q, __builtin_elementwise_maximum(z, 0.0f));
+}
+
 // act(v) in place.  relu passes a NaN on, as the others do.
 template <int N>
 __device__ inline void activate(float (&v)[N], int act) {
@@ -130,7 +153,11 @@ __device__ inline void activate(float (&v)[N], int act) {
         for (int e = 0; e < N; ++e) v[e] = v[e] < 0.0f ? 0.0f : v[e];
     } else if (act == JH_ACT_GELU) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) v[e] = gelu_erf(v[e]);
+        for (int i = 0; i < N; ++i) {
+            float a, e;
+            const float q = normal_tail(v[i], a, e);
+            v[i] = gelu_of(v[i], a, q);
+        }
     } else if (act == JH_ACT_SILU) {
 #pragma unroll
         for (int e = 0; e < N; ++e) v[e] *= sigmoid(v[e]);
