@@ -460,6 +460,7 @@ __device__ inline void finish_gated8(const LinearArgs& a, float (&g)[8], float (
 template <class T, int LAYOUT, int EPI, int NJ, int HALF, bool EARLY>
 struct Epilogue {
     static constexpr int AHEAD = EARLY || NJ < 4 ? NJ : 4;
+    static constexpr bool TERMS = LAYOUT == ROWS_ROWS;  // gradients are the sums alone
     const LinearArgs& a;
     int t0, c0, lane;
     ColumnTerms<T> col[2];
@@ -473,7 +474,7 @@ struct Epilogue {
     __device__ int first_row(int j) const { return t0 + (j < HALF ? j * 16 : 128 + (j - HALF) * 16); }
     __device__ int row(int j) const { return first_row(j) + (lane & 15); }
     __device__ void load_columns() {
-        if (a.partial) return;
+        if (!TERMS) return;
         col[0].load(a, c0, a.p_scale);
         if constexpr (EPI == EPI_GATED) col[1].load(a, c0, a.p_scale ? a.p_scale + a.p_cols : nullptr);
         else col[1].load(a, c0 + 8, a.p_scale);
@@ -483,7 +484,7 @@ struct Epilogue {
         }
     }
     __device__ void load_residuals(int j) {  // of row blocks j .. j + AHEAD - 1
-        if (EPI == EPI_GATED || !a.resid) return;
+        if (!TERMS || EPI == EPI_GATED || !a.resid) return;
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i)
             if (j + i < NJ) resid[i].load(a, first_row(j + i), c0, lane);
@@ -508,20 +509,24 @@ struct Epilogue {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) z[e >> 3][e & 7] = c[e >> 2][e & 3];
                 const long first = first_row(j);
-                if (a.partial) {
+                if (!TERMS && a.partial) {
                     store_f32(a.partial + (long)split * a.q_rows * a.p_cols, a.p_cols, first, c0, lane, a.q_rows, a.p_cols, z);
                 } else {
+                    if constexpr (TERMS) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) col[h].apply(a, z[h], qs);
-                    if constexpr (T::bytes == 2)
+                        for (int h = 0; h < 2; ++h) col[h].apply(a, z[h], qs);
+                    }
+                    if constexpr (TERMS && T::bytes == 2)
                         if (a.pre) store_half<T>(a.pre, a.ldpre, first, c0, lane, a.q_rows, a.p_cols, z);
+                    if constexpr (TERMS) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) activate(z[h], a.act);
+                        for (int h = 0; h < 2; ++h) activate(z[h], a.act);
+                    }
                     if (!ResidLines<T>::HALF_ONLY && a.out_f32) {
-                        if (a.resid) resid[j % AHEAD].add_f32(z);
+                        if (TERMS && a.resid) resid[j % AHEAD].add_f32(z);
                         store_f32(a.out, a.ldo, first, c0, lane, a.q_rows, a.p_cols, z);
                     } else {
-                        if (a.resid) resid[j % AHEAD].add_half(z);
+                        if (TERMS && a.resid) resid[j % AHEAD].add_half(z);
                         store_half<T>(a.out, a.ldo, first, c0, lane, a.q_rows, a.p_cols, z);
                     }
                 }
