@@ -275,7 +275,8 @@ enum {
  * scales[rows]: scale = max|out| / 448 per row, and each code is the e4m3 value
  * nearest to the exact quotient of 448 s w by its row's max|s w| (ties to even),
  * so that codes do not depend on how sums are ordered.  A row of zeros has scale
- * 0; a NaN gives NaN codes; a row with an infinity has no finite scale.
+ * 0, whatever eps (its 16-bit output with eps = 0 is 0 / 0); a NaN gives NaN codes; a row
+ * with an infinity has no finite scale.
  * rstd[rows] (or NULL) receives 1 / sqrt(mean(s^2) + eps) for the backward pass.
  */
 int jh_op_rms_norm(int x_type, const void* x, size_t ldx, int resid_type, const void* resid, size_t ldr,

@@ -241,7 +241,8 @@ __global__ __launch_bounds__(THREADS) void rms_norm_kernel(RmsNormArgs a) {
             for (int e = 0; e < 8; ++e) m = fmax(m, fabs((double)s[c][e] * (double)w[c][e]));
         m = row_max<TPR>(m, max_slot);
         const double inv = m > 0.0 ? 1.0 / m : 0.0;
-        if (lane == 0) a.scales[row] = (float)(m * (double)r / 448.0);
+        // a row of zeros has scale 0 with eps = 0 too, where r is infinite
+        if (lane == 0) a.scales[row] = m > 0.0 || r != r ? (float)(m * (double)r / 448.0) : 0.0f;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int i = (c * TPR + lane) * 8;
