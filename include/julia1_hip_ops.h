@@ -258,7 +258,8 @@ enum {
  * current device's, whose stream the call is put on; nothing is allocated, so calls
  * can be captured into graphs.  A workspace is scratch of one call at a time: calls
  * that may run at once, replays of graphs among them, have one each.  Sums,
- * statistics and activations are FP32, results are rounded once, and every sum
+ * statistics and activations are FP32 (but for sums of e4m3 products with a bf16 output,
+ * see jh_op_linear), results are rounded once, and every sum
  * has a fixed order: the same call gives the same bits.  GELU and SiLU are good to
  * (8 + E) 2^-23 of their value, E = z^2 and |z| (the tanh form: 4 times the argument
  * of its exponential), down to 2^-119.  A row's bits may depend
@@ -314,9 +315,12 @@ int jh_op_quantize_rows(int x_type, const void* x, size_t ldx, size_t rows, size
  * x_scale[rows] and w_scale[n] belong to e4m3 (NULL: ones); bias f32 [n] or NULL.
  * out and resid (or NULL) have out_type: f32, or type (bf16 for e4m3); resid may
  * be out itself, with its stride.  pre [rows, n] of type (16-bit types; or NULL)
- * receives z for the backward pass.  With e4m3 operands and a bf16 output the sums
- * carry the 8-bit matrix instruction's own error, 1.5e-5 of their norm (1/100 of the
- * rounding to bf16); with an f32 output they are FP32 sums of exact products.
+ * receives z for the backward pass.  With e4m3 operands and a bf16 output the 8-bit
+ * matrix instruction drops of every product the bits below 2^-13 of the largest one that it
+ * adds with it: a sum is off by less than k 2^-13 of its largest |x w|, so where large
+ * products cancel, small ones may be lost whole.  (Of normally distributed operands sums
+ * came out within 1.5e-5 of their norm, 1/100 of the rounding to bf16.)  With an f32 output they
+ * are FP32 sums of exact products, at half the rate.
  */
 int jh_op_linear(int type, const void* x, size_t ldx, const float* x_scale, size_t rows, const void* w,
                  const float* w_scale, size_t n, size_t k, const float* bias, int act, const void* resid,
@@ -340,7 +344,8 @@ size_t jh_op_linear_backward_workspace(size_t rows, size_t n, size_t k, int act)
 /*
  * out = act(x Wg^T) * (x Wu^T) in one kernel: wi [2 inter, k] holds Wg's rows and then
  * Wu's, as jh_encoder_layer.wi does (JH_EPI_GEGLU_BF16's interleave is not needed).
- * type as for jh_op_linear, wi_scale [2 inter]; out has type (bf16 for e4m3).  gu
+ * type as for jh_op_linear, wi_scale [2 inter]; out has type (bf16 for e4m3, whose sums
+ * are as jh_op_linear's with a bf16 output).  gu
  * [rows, 2 inter] of type (16-bit types; or NULL) receives both projections for
  * the backward pass.
  */
