@@ -375,13 +375,12 @@ size_t jh_op_gated_ffn_backward_workspace(size_t rows, size_t inter, size_t k);
  */
 enum { JH_PRODUCT_LINEAR = 0, JH_PRODUCT_GATED = 1, JH_PRODUCT_DX = 2, JH_PRODUCT_DW = 3 };
 enum {
-    JH_KERNEL_SMALL = 0,   /* 64 x 64 tiles                                           */
-    JH_KERNEL_GROUP = 1,   /* 64 x 64, four groups of waves share the contraction     */
-    JH_KERNEL_DEEP = 2,    /* 128 x 128, one tile to a CU                             */
-    JH_KERNEL_PAIR = 3,    /* 128 x 128, two to a CU                                  */
-    JH_KERNEL_TALL = 4,    /* 256 rows x 128 columns                                  */
-    JH_KERNEL_WIDE = 5,    /* 256 x 256                                               */
-    JH_KERNEL_STREAM = 6   /* up to 16 rows, w streams past them                      */
+    JH_KERNEL_SMALL = 0,   /* 64 x 64 tiles                            */
+    JH_KERNEL_DEEP = 1,    /* 128 x 128, one tile to a CU              */
+    JH_KERNEL_PAIR = 2,    /* 128 x 128, two to a CU                   */
+    JH_KERNEL_TALL = 3,    /* 256 rows x 128 columns                   */
+    JH_KERNEL_WIDE = 4,    /* 256 x 256                                */
+    JH_KERNEL_STREAM = 5   /* up to 16 rows, w streams past them       */
 };
 typedef struct {
     int kernel, parts;

@@ -253,7 +253,7 @@ LinearPlan linear_plan(int product, int type, int out_type, size_t rows, size_t 
 
 // One kernel each: 256 x 256 tiles, smaller tiles, and few rows.
 void launch_linear_wide(const LinearArgs& a, hipStream_t stream);  // not e4m3 operands with an FP32 output
-enum class LinearTile { Small, Group, Deep, Pair, Tall };  // see linear_tile.hip
+enum class LinearTile { Small, Deep, Pair, Tall };  // see linear_tile.hip
 void launch_linear_tile(const LinearArgs& a, LinearTile tile, hipStream_t stream);
 void launch_linear_small(const LinearArgs& a, hipStream_t stream);  // at most 16 rows, k contiguous
 

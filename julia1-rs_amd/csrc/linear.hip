@@ -167,24 +167,34 @@ long tiles_of(const LinearArgs& a, int p, int q) {
 
 // What a launch of each kernel takes, in us, from its number of tiles and of K steps: a start
 // and an end per round of tiles (launch, first loads, epilogue) and a time per step that grows
-// with the CUs at work (shared L2 and power).  The constants are fits to times of products on an
-// MI355X (256 CUs), the inputs in three sets that take turns, as a layer meets its own; of 86
-// sizes (633 ways to run them) the kernel that comes out cheapest takes 0.3 % longer than the
-// fastest in the mean, 11 % at worst.  Some of them, bf16 (us, the kernel taken in brackets):
+// with the CUs at work (shared L2 and power).  The constants are fits to times on an MI355X (256 CUs):
+// products to 86 sizes whose inputs, in three sets, take turns, as a layer meets its own (of 633
+// ways to run them the kernel that comes out cheapest takes 0.3 % longer than the fastest in the
+// mean, 11 % at worst); gradients to 100 sizes, log-uniform and training widths by turns, with as many sets of
+// inputs as 700 MB hold, so that none is left in the 256 MB of cache (0.7 % and 21 %; on 140
+// other sizes 1.5 % and 25 %).  Some of them, bf16, gradients in their best number of parts (us, the
+// kernel taken in brackets):
 //
-//   rows x n x k              Small   Group   Deep    Pair    Tall    256 x 256
-//   512 x 768 x 768           [7.0]           9.9     12.2    13.8    21.2
-//   1024 x 1024 x 4096        [19.9]          30.4    51.3    45.1    70.7
-//   1024 x 4096 x 1024        19.5            [14.3]  19.4    18.4    26.2
-//   9482 x 768 x 1152         32.3            27.1    25.4    [21.8]  29.6
-//   2048 x 4096 x 4096        111             71.6    68.6    [59.9]  74.9
-//   4096 x 4096 x 4096        204             143     135     121     [101]
-//   9482 x 4096 x 1024        147             111     99.8    96.6    [88.3]
-//   dx of 1024 x 4096 x 1024  25.5    [22.3]  37.7    50.7            78.4
-//   dx of 9482 x 2304 x 768   70.1    91.0    48.2    [37.4]          50.0
-//   dw of 4096 x 4096 x 1024  66.1    78.7    [40.0]  50.2            98.2
-//   dw of 8192 x 4096 x 4096  527     742     340     264             [223]
-enum { SMALL = JH_KERNEL_SMALL, GROUP = JH_KERNEL_GROUP, DEEP = JH_KERNEL_DEEP, PAIR = JH_KERNEL_PAIR, TALL = JH_KERNEL_TALL,
+//   rows x n x k              Small   Deep    Pair    Tall    256 x 256
+//   512 x 768 x 768           [7.0]   9.9     12.2    13.8    21.2
+//   1024 x 1024 x 4096        [19.9]  30.4    51.3    45.1    70.7
+//   1024 x 4096 x 1024        19.5    [14.3]  19.4    18.4    26.2
+//   9482 x 768 x 1152         32.3    27.1    25.4    [21.8]  29.6
+//   2048 x 4096 x 4096        111     71.6    68.6    [59.9]  74.9
+//   4096 x 4096 x 4096        204     143     135     121     [101]
+//   9482 x 4096 x 1024        147     111     99.8    96.6    [88.3]
+//   dx of 4096 x 1024 x 768   18.8    [16.3]  19.5            27.8
+//   dx of 9482 x 2304 x 768   70.5    59.7    [44.0]          51.8
+//   dx of 9482 x 1152 x 4096  172     134     102             [95.6]
+//   dw of 1024 x 4096 x 1024  23.6    [17.0]  19.8            31.7
+//   dw of 4096 x 4096 x 1024  74.1    [48.4]  51.1            54.7
+//   dw of 9482 x 2048 x 768   76.3    62.7    52.3            [53.7]
+//   dw of 16384 x 2304 x 1024 171     134     101             [92.1]
+//   dw of 8192 x 4096 x 8192  1006    622     502             [440]
+//
+// (64 x 64 tiles of which four groups of waves shared the contraction were the fastest in none of these
+// 240 sizes: 18.2 us for dw of 1024 x 768 x 2048, Small 13.0.)
+enum { SMALL = JH_KERNEL_SMALL, DEEP = JH_KERNEL_DEEP, PAIR = JH_KERNEL_PAIR, TALL = JH_KERNEL_TALL,
        WIDE = JH_KERNEL_WIDE, KERNELS };
 constexpr long CUS = 256;
 
@@ -199,24 +209,18 @@ double cost(int kernel, const LinearArgs& a, long splits) {
     switch (kernel) {
         case SMALL: {
             const long t = tiles_of(a, 64, 64) * splits;
-            if (t <= CUS) return 3.7 + (by_cols ? 0.33 : 0.215 + 0.05 * load((double)t)) * s;
-            return rounds(t, 2 * CUS, [&](double) { return 0.42 * s + 2.0; }) + (by_cols ? 5.0 : 1.0);
-        }
-        case GROUP: {
-            const long t = tiles_of(a, 64, 64) * splits;
-            return rounds(t, CUS, [&](double) { return std::ceil(s / 4) + 5.0; }) + 1.5;
+            if (by_cols) return t <= CUS ? 3.4 + 0.4 * s : rounds(t, 2 * CUS, [&](double) { return 0.53 * s + 1.5; }) + 3.7;
+            if (t <= CUS) return 3.7 + (0.215 + 0.05 * load((double)t)) * s;
+            return rounds(t, 2 * CUS, [&](double) { return 0.42 * s + 2.0; }) + 1.0;
         }
         case DEEP: {
             const long t = tiles_of(a, 128, 128) * splits;
-            // operands well past the L2s' 32 MB come late for its two steps per group in flight (dw of
-            // 9482 x 1024 x 4096, 97 MB, in one part: 83 us of inputs read just before, 104 of others;
-            // Pair in two parts 92 and 99.  9482 x 1024 x 768, 34 MB, in four parts: 35 and 35)
-            const double far = ((double)a.q_rows + a.p_cols) * a.k * 2 > 48e6 ? 0.13 : 0.0;
-            if (by_cols) return rounds(t, CUS, [&](double n) { return s * (0.49 + (0.05 + far) * load(n)) + 4.0; }) + 1.0;
+            if (by_cols) return rounds(t, CUS, [&](double) { return 0.71 * s + 3.4; }) + 3.4;
             return rounds(t, CUS, [&](double n) { return s * (0.35 + 0.19 * load(n)) + 3.0; }) + 1.5;
         }
         case PAIR: {
             const long t = tiles_of(a, 128, 128) * splits;
+            if (by_cols) return rounds(t, 2 * CUS, [&](double n) { return s * (n > CUS ? 1.07 : 0.78 + 0.24 * load(n)) + 3.8; }) + 2.5;
             return rounds(t, 2 * CUS, [&](double n) { return s * (n > CUS ? 0.92 : 0.62 + 0.16 * load(n)) + 5.0; }) + 1.0;
         }
         case TALL: {
@@ -225,9 +229,9 @@ double cost(int kernel, const LinearArgs& a, long splits) {
         }
         default: {
             const long t = tiles_of(a, 256, 256) * splits;
-            const double alone = a.layout == COLS_COLS ? 1.37 : by_cols ? 1.0 : 0.88;
-            const double all = a.layout == COLS_COLS ? 1.57 : by_cols ? 1.45 : 1.37;
-            return rounds(t, CUS, [&](double n) { return s * (alone + (all - alone) * load(n) * load(n)) + 9.0; }) + 1.0;
+            const double alone = a.layout == COLS_COLS ? 1.35 : by_cols ? 1.25 : 0.88;
+            const double all = a.layout == COLS_COLS ? 1.56 : by_cols ? 1.51 : 1.37;
+            return rounds(t, CUS, [&](double n) { return s * (alone + (all - alone) * load(n) * load(n)) + (by_cols ? 9.5 : 9.0); }) + 1.0;
         }
     }
 }
@@ -235,8 +239,8 @@ double cost(int kernel, const LinearArgs& a, long splits) {
 // Whether a launch can hold the kernel's tiles along x, where it has fewer than 2^32 threads.  (2^30 rows
 // by 8 columns: 2^24 tiles of 64 x 64 by 256 threads are too many, 2^23 of 128 x 128 are not.)
 bool launches(int kernel, const LinearArgs& a) {
-    const int side = kernel == WIDE ? 256 : kernel == SMALL || kernel == GROUP ? 64 : 128;
-    const long threads = kernel == GROUP ? 1024 : kernel == SMALL || kernel == PAIR ? 256 : 512;
+    const int side = kernel == WIDE ? 256 : kernel == SMALL ? 64 : 128;
+    const long threads = kernel == SMALL || kernel == PAIR ? 256 : 512;
     return tiles_of(a, side, kernel == TALL ? 256 : side) * threads < 1L << 32;
 }
 
@@ -256,15 +260,12 @@ Choice pick(const LinearArgs& a, bool gradient) {
     const double out = (double)a.q_rows * a.p_cols * 4;
     for (long splits = 1; splits <= (gradient ? MAX_SPLITS : 1); splits += splits < 4 ? 1 : splits < 8 ? 2 : 4) {
         if (splits > 1 && (steps_of(a) < splits * MIN_STEPS || out * splits > split_bytes(a))) break;
-        const double sum = splits > 1 ? 2.5 + (2 * splits + 0.5) * out / 5e6 : 0.0;  // written and read
+        const double sum = splits > 1 ? 4.5 + (2 * splits + 0.5) * out / 9e6 : 0.0;  // written and read, mostly in cache
         for (int kernel = 0; kernel < KERNELS; ++kernel) {
             // no room there for e4m3 fragments widened to bf16; Tall gains nothing by columns (9482 x 768
             // x 2304: 38.2 us, Pair 37.5)
             if (kernel >= TALL && a.type == JH_E4M3 && a.out_f32) continue;
             if (kernel == TALL && a.layout != ROWS_ROWS) continue;
-            // The groups share a long contraction; k contiguous that gains only where both operands are
-            // in L2 already (128 x 1024 x 4096: 15.1 us against Small's 17.5, else 20.0 against 17.7)
-            if (kernel == GROUP && a.layout == ROWS_ROWS) continue;
             if (!launches(kernel, a)) continue;
             const double c = cost(kernel, a, splits) + sum;
             if (c < best.cost) best = {kernel, (int)splits, c};
@@ -330,8 +331,8 @@ long partial_bytes(const LinearArgs& a, const Plan& p) {
 void launch(int kernel, const LinearArgs& a, hipStream_t s) {
     if (kernel == JH_KERNEL_STREAM) launch_linear_small(a, s);
     else if (kernel == WIDE) launch_linear_wide(a, s);
-    else launch_linear_tile(a, kernel == SMALL ? LinearTile::Small : kernel == GROUP ? LinearTile::Group
-                               : kernel == DEEP ? LinearTile::Deep : kernel == PAIR ? LinearTile::Pair : LinearTile::Tall, s);
+    else launch_linear_tile(a, kernel == SMALL ? LinearTile::Small : kernel == DEEP ? LinearTile::Deep
+                               : kernel == PAIR ? LinearTile::Pair : LinearTile::Tall, s);
 }
 
 template <class T>

@@ -3,8 +3,6 @@
 // stages of LDS, NST steps (of every group) ahead.
 //
 //   Small  64 x 64, 4 waves, 4 stages (64 KB)
-//   Group  64 x 64, 4 groups of 4 waves, 2 stages (128 KB): a quarter of the steps, one
-//          after the other, for few tiles of long contractions by columns
 //   Deep   128 x 128, one tile per CU (128 KB): 8 waves and 4 stages where k is contiguous;
 //          2 groups of 4 waves and 2 stages where an operand lies by columns, as a transposing
 //          read brings half as much and waves of 64 x 64 read less (a contraction of 9482 into
@@ -32,7 +30,7 @@ using namespace lin;
 namespace {
 
 template <class T, int LAYOUT, int EPI, int WP, int WQ, int NJ, int KG, int NST>
-__global__ __launch_bounds__(64 * WP * WQ * KG) __attribute__((amdgpu_waves_per_eu(WP * WQ * KG == 16 ? 4 : 2))) void linear_tile_kernel(LinearArgs a) {
+__global__ __launch_bounds__(64 * WP * WQ * KG) __attribute__((amdgpu_waves_per_eu(2))) void linear_tile_kernel(LinearArgs a) {
     constexpr int TP = 64 * WP, TQ = 16 * NJ * WQ;                       // operand rows of a tile
     constexpr int SUB = (TP + TQ) * STEP_BYTES, STAGE = KG * SUB, Q_AT = TP * STEP_BYTES;
     constexpr int PI = 8 / WQ, QI = 2 * NJ / WP;                         // 1 KB DMA instructions per wave and stage
@@ -206,8 +204,7 @@ void launch(const LinearArgs& a, LinearTile tile, hipStream_t s) {
     if (tile == LinearTile::Small) launch_tiles<T, LAYOUT, EPI, 1, 4, 1, 1, 4>(a, s);
     else if (tile == LinearTile::Pair) launch_tiles<T, LAYOUT, EPI, 2, 2, 4, 1, 2>(a, s);
     else if constexpr (LAYOUT != ROWS_ROWS) {
-        if (tile == LinearTile::Group) launch_tiles<T, LAYOUT, EPI, 1, 4, 1, 4, 2>(a, s);
-        else launch_tiles<T, LAYOUT, EPI, 2, 2, 4, 2, 2>(a, s);
+        launch_tiles<T, LAYOUT, EPI, 2, 2, 4, 2, 2>(a, s);
     } else if (std::is_same_v<T, E4m3Wide> || tile == LinearTile::Deep) launch_tiles<T, LAYOUT, EPI, 2, 4, 2, 1, 4>(a, s);
     else if constexpr (!std::is_same_v<T, E4m3Wide>) launch_tiles<T, LAYOUT, EPI, 2, 4, 4, 1, 3>(a, s);
 }

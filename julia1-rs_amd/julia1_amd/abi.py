@@ -37,7 +37,7 @@ F32, BF16, F16, E4M3 = range(4)
 ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = range(5)
 # products and kernels of jh_op_linear_plan
 PRODUCT_LINEAR, PRODUCT_GATED, PRODUCT_DX, PRODUCT_DW = range(4)
-KERNEL_SMALL, KERNEL_GROUP, KERNEL_DEEP, KERNEL_PAIR, KERNEL_TALL, KERNEL_WIDE, KERNEL_STREAM = range(7)
+KERNEL_SMALL, KERNEL_DEEP, KERNEL_PAIR, KERNEL_TALL, KERNEL_WIDE, KERNEL_STREAM = range(6)
 
 _f32p = C.POINTER(C.c_float)
 

@@ -555,7 +555,7 @@ def linear_plan(product, dtype, rows, n, k, out_dtype=None):
     out = codes[out_dtype] if out_dtype is not None else abi.BF16 if t == abi.E4M3 else t
     launches = (LinearLaunch * 2)()
     check(lib().jh_op_linear_plan(("linear", "gated", "dx", "dw").index(product), t, out, rows, n, k, launches))
-    names = ("small", "group", "deep", "pair", "tall", "wide", "stream")
+    names = ("small", "deep", "pair", "tall", "wide", "stream")
     return [(names[v.kernel], v.parts, v.rows) for v in launches if v.parts]
 
 

@@ -6,8 +6,9 @@ torch = pytest.importorskip("torch")
 from julia1_amd import abi, hip  # noqa: E402
 
 BF16, F16, F32, E4M3 = torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3fn
-TILE = {"small": (64, 64, 256), "group": (64, 64, 1024), "deep": (128, 128, 512), "pair": (128, 128, 256),
-        "tall": (128, 256, 512), "wide": (256, 256, 512)}  # columns and rows of a tile, threads
+# columns and rows of a tile, threads
+TILE = {"small": (64, 64, 256), "deep": (128, 128, 512), "pair": (128, 128, 256),
+        "tall": (128, 256, 512), "wide": (256, 256, 512)}
 
 
 def threads(product, launch, cols):
@@ -75,3 +76,11 @@ def test_plan_refusals(change):
                 launches=(hip.LinearLaunch * 2)())
     assert hip.lib().jh_op_linear_plan(*base.values()) == abi.JH_OK
     assert hip.lib().jh_op_linear_plan(*{**base, **change}.values()) == abi.JH_ERR_INVALID
+
+
+@pytest.mark.parametrize("n,k", [(1024, 1024), (1024, 4096), (4096, 1024), (2304, 768), (4096, 4096), (264, 5000)])
+def test_a_contraction_is_planned_by_its_steps(n, k):
+    """dw's contraction runs in steps of 64 rows, whose number decides the kernel and the parts; no other border does."""
+    for step in range(1, 520):
+        plans = {tuple(hip.linear_plan("dw", BF16, 64 * step - i, n, k)) for i in (63, 40, 1, 0)}
+        assert len(plans) == 1, (step, plans)
