@@ -1,8 +1,12 @@
 """The kernels that products are put on by their sizes, asked from the library: no device is needed."""
+import math
+import random
+
 import pytest
 
 torch = pytest.importorskip("torch")
 
+from ffn_routes import ROUTES, route  # noqa: E402
 from julia1_amd import abi, hip  # noqa: E402
 
 BF16, F16, F32, E4M3 = torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3fn
@@ -84,3 +88,30 @@ def test_a_contraction_is_planned_by_its_steps(n, k):
     for step in range(1, 520):
         plans = {tuple(hip.linear_plan("dw", BF16, 64 * step - i, n, k)) for i in (63, 40, 1, 0)}
         assert len(plans) == 1, (step, plans)
+
+
+TYPES = {"half": (BF16, None), "e4m3": (E4M3, None), "e4m3 to f32": (E4M3, F32)}
+
+
+@pytest.mark.parametrize("product,types", list(ROUTES))
+def test_sizes_of_every_route(product, types):
+    """The sizes that other tests take for a kernel run on it, in both 16-bit types."""
+    dtype, out = TYPES[types]
+    for name, size in ROUTES[product, types].items():
+        assert route(hip.linear_plan(product, dtype, *size, out)) == name, (name, size)
+        if types == "half":
+            assert route(hip.linear_plan(product, F16, *size, F32 if product in ("linear", "dw") else None)) == name
+
+
+@pytest.mark.parametrize("product,types", list(ROUTES))
+def test_no_other_route(product, types):
+    """Sizes drawn over the whole range (up to what a card trains on) take none that is not listed."""
+    dtype, out = TYPES[types]
+    rng = random.Random(5)
+
+    def draw(lo, hi, step):
+        return max(step, int(math.exp(rng.uniform(math.log(lo), math.log(hi)))) // step * step)
+
+    for _ in range(6000):
+        size = draw(1, 40000, 1), draw(8, 9000, 8), draw(16, 9000, 16)
+        assert route(hip.linear_plan(product, dtype, *size, out)) in ROUTES[product, types], size
