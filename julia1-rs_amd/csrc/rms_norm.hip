@@ -11,9 +11,11 @@
 //   quantize_rows      8192 x 8192 f32                              336 MB   62.9 us  5.3 TB/s
 //   quantize_rows      9482 x 1152 bf16                              33 MB    9.3 us  3.5 TB/s (1)
 //   rms_norm_backward  16384 x 4096 bf16, with dres and dw          537 MB   98.5 us  5.4 TB/s
+//   rms_norm_backward  4096 x 16384 bf16, with dres and dw          537 MB    117 us  4.6 TB/s (2)
 //   column_sum         512 x 4096, of that dw's parts                 8 MB    4.9 us
 //
 //   (1) a launch (2 us) and the codes' arithmetic count here: 12.7 us with codes formed in 64 bits
+//   (2) one wave per SIMD, so that a row's loads and sums are not under another's; dw's sum included
 //
 //   forward   s = x + resid, rounded to the residual's type (what is stored is what is
 //             normalised); r = 1 / sqrt(mean(s^2) + eps); y = s r w
@@ -503,10 +505,13 @@ void check_codes(const char* op, const void* q, size_t ld, size_t rows, size_t c
     if (ld > ((size_t)1 << 22)) refuse(op, "the e4m3 output: row stride over 4 MiB");
 }
 
-// Workgroups of the backward pass, each with a part of dw: two per CU, fewer where there
-// are fewer rows than they hold at once.
+// Workgroups of the backward pass, each with a part of dw: as many as the GPU holds at once, fewer where
+// there are fewer rows than they take.  That is two per CU of up to 8192 columns, one of more, whose
+// six or eight chunks per thread need over 256 registers.  (One and two per CU, bf16 with dres and dw:
+// 16384 x 4096 111 and 104 us, 8192 x 8192 108 and 108, 5461 x 12288 111 and 117, 4096 x 16384 117
+// and 127, 300 x 16384 22 and 26.)
 int backward_blocks(int rows, int hidden) {
-    return std::max(1, std::min(row_blocks(rows, hidden <= 2048 ? 64 : 256), 512));
+    return std::max(1, std::min(row_blocks(rows, hidden <= 2048 ? 64 : 256), hidden <= 8192 ? 512 : 256));
 }
 
 }  // namespace

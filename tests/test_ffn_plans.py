@@ -115,3 +115,10 @@ def test_no_other_route(product, types):
     for _ in range(6000):
         size = draw(1, 40000, 1), draw(8, 9000, 8), draw(16, 9000, 16)
         assert route(hip.linear_plan(product, dtype, *size, out)) in ROUTES[product, types], size
+
+
+def test_norm_gradient_workgroups_fit_the_gpu():
+    """A part of dw per workgroup that the 256 CUs hold at once: two each up to 8192 columns, one of longer rows."""
+    for hidden, most in ((8, 512), (2056, 512), (8192, 512), (8200, 256), (16384, 256)):
+        assert hip.rms_norm_backward_workspace(100000, hidden) == most * hidden * 4
+    assert hip.rms_norm_backward_workspace(200, 16384) == 200 * 16384 * 4
