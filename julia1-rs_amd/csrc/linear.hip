@@ -170,10 +170,10 @@ long tiles_of(const LinearArgs& a, int p, int q) {
 // with the CUs at work (shared L2 and power).  The constants are fits to times on an MI355X (256 CUs):
 // products to 86 sizes whose inputs, in three sets, take turns, as a layer meets its own (of 633
 // ways to run them the kernel that comes out cheapest takes 0.3 % longer than the fastest in the
-// mean, 11 % at worst); gradients to 100 sizes, log-uniform and training widths by turns, with as many sets of
-// inputs as 700 MB hold, so that none is left in the 256 MB of cache (0.7 % and 21 %; on 140
-// other sizes 1.5 % and 25 %).  Some of them, bf16, gradients in their best number of parts (us, the
-// kernel taken in brackets):
+// mean, 11 % at worst); gradients to 124 sizes, log-uniform ones and training widths, with as many
+// sets of inputs as 700 MB hold, so that none is left in the 256 MB of cache, but dz just written, as the
+// activation's gradient leaves it (0.6 % and 11 %; on 140 other sizes 1.1 % and 18 %).  Some of them,
+// bf16, gradients in their best number of parts (us, the kernel taken in brackets):
 //
 //   rows x n x k              Small   Deep    Pair    Tall    256 x 256
 //   512 x 768 x 768           [7.0]   9.9     12.2    13.8    21.2
@@ -183,24 +183,25 @@ long tiles_of(const LinearArgs& a, int p, int q) {
 //   2048 x 4096 x 4096        111     71.6    68.6    [59.9]  74.9
 //   4096 x 4096 x 4096        204     143     135     121     [101]
 //   9482 x 4096 x 1024        147     111     99.8    96.6    [88.3]
-//   dx of 4096 x 1024 x 768   18.8    [16.3]  19.5            27.8
-//   dx of 9482 x 2304 x 768   70.5    59.7    [44.0]          51.8
-//   dx of 9482 x 1152 x 4096  172     134     102             [95.6]
-//   dw of 1024 x 4096 x 1024  23.6    [17.0]  19.8            31.7
-//   dw of 4096 x 4096 x 1024  74.1    [48.4]  51.1            54.7
-//   dw of 9482 x 2048 x 768   76.3    62.7    52.3            [53.7]
-//   dw of 16384 x 2304 x 1024 171     134     101             [92.1]
-//   dw of 8192 x 4096 x 8192  1006    622     502             [440]
+//   dx of 4096 x 1024 x 768   18.6    [15.5]  18.8            27.2
+//   dx of 9482 x 2304 x 768   65.9    48.9    [42.5]          49.9
+//   dx of 9482 x 1152 x 4096  178     143     107             [102]
+//   dw of 1024 x 4096 x 1024  23.3    [16.3]  19.3            31.1
+//   dw of 4096 x 4096 x 1024  70.6    [45.1]  48.2            53.6
+//   dw of 8192 x 1152 x 2048  92.9    75.0    [58.9]          61.3
+//   dw of 9482 x 2304 x 768   73.8    58.7    51.8            [54.6]
+//   dw of 16384 x 2304 x 1024 162     122     96.4            [90.3]
+//   dw of 8192 x 4096 x 8192  1024    637     535             [461]
 //
-// (64 x 64 tiles of which four groups of waves shared the contraction were the fastest in none of these
-// 240 sizes: 18.2 us for dw of 1024 x 768 x 2048, Small 13.0.)
+// (64 x 64 tiles of which four groups of waves shared the contraction were the fastest in none of 240
+// sizes: 18.2 us for dw of 1024 x 768 x 2048, Small 13.0.)
 enum { SMALL = JH_KERNEL_SMALL, DEEP = JH_KERNEL_DEEP, PAIR = JH_KERNEL_PAIR, TALL = JH_KERNEL_TALL,
        WIDE = JH_KERNEL_WIDE, KERNELS };
 constexpr long CUS = 256;
 
 double cost(int kernel, const LinearArgs& a, long splits) {
     const double s = (double)((steps_of(a) + splits - 1) / splits);
-    const bool by_cols = a.layout != ROWS_ROWS;
+    const bool by_cols = a.layout != ROWS_ROWS, both = a.layout == COLS_COLS;
     // `of(n)`: a round of n tiles, `slots` of which the GPU holds
     auto rounds = [](long t, long slots, auto of) {
         return (double)(t / slots) * of((double)slots) + (t % slots ? of((double)(t % slots)) : 0.0);
@@ -209,18 +210,22 @@ double cost(int kernel, const LinearArgs& a, long splits) {
     switch (kernel) {
         case SMALL: {
             const long t = tiles_of(a, 64, 64) * splits;
-            if (by_cols) return t <= CUS ? 3.4 + 0.4 * s : rounds(t, 2 * CUS, [&](double) { return 0.53 * s + 1.5; }) + 3.7;
+            if (by_cols && t <= CUS) return 3.9 + 0.36 * s;
+            if (by_cols) return rounds(t, 2 * CUS, [&](double) { return (both ? 0.5 : 0.47) * s + 1.6; }) + 4.1;
             if (t <= CUS) return 3.7 + (0.215 + 0.05 * load((double)t)) * s;
             return rounds(t, 2 * CUS, [&](double) { return 0.42 * s + 2.0; }) + 1.0;
         }
         case DEEP: {
             const long t = tiles_of(a, 128, 128) * splits;
-            if (by_cols) return rounds(t, CUS, [&](double) { return 0.71 * s + 3.4; }) + 3.4;
+            if (by_cols) return rounds(t, CUS, [&](double) { return (both ? 0.63 : 0.61) * s + 4.1; }) + 3.2;
             return rounds(t, CUS, [&](double n) { return s * (0.35 + 0.19 * load(n)) + 3.0; }) + 1.5;
         }
         case PAIR: {
             const long t = tiles_of(a, 128, 128) * splits;
-            if (by_cols) return rounds(t, 2 * CUS, [&](double n) { return s * (n > CUS ? 1.07 : 0.78 + 0.24 * load(n)) + 3.8; }) + 2.5;
+            if (by_cols) {
+                const double full = both ? 1.03 : 1.05, alone = both ? 0.75 : 0.7;
+                return rounds(t, 2 * CUS, [&](double n) { return s * (n > CUS ? full : alone + 0.16 * load(n)) + 4.9; }) + 1.8;
+            }
             return rounds(t, 2 * CUS, [&](double n) { return s * (n > CUS ? 0.92 : 0.62 + 0.16 * load(n)) + 5.0; }) + 1.0;
         }
         case TALL: {
@@ -229,9 +234,9 @@ double cost(int kernel, const LinearArgs& a, long splits) {
         }
         default: {
             const long t = tiles_of(a, 256, 256) * splits;
-            const double alone = a.layout == COLS_COLS ? 1.35 : by_cols ? 1.25 : 0.88;
-            const double all = a.layout == COLS_COLS ? 1.56 : by_cols ? 1.51 : 1.37;
-            return rounds(t, CUS, [&](double n) { return s * (alone + (all - alone) * load(n) * load(n)) + (by_cols ? 9.5 : 9.0); }) + 1.0;
+            const double alone = both ? 1.28 : by_cols ? 1.04 : 0.88, all = both ? 1.62 : by_cols ? 1.51 : 1.37;
+            return rounds(t, CUS, [&](double n) { return s * (alone + (all - alone) * load(n) * load(n)) + (by_cols ? 11.1 : 9.0); }) +
+                   (by_cols ? 0.0 : 1.0);
         }
     }
 }
@@ -260,7 +265,7 @@ Choice pick(const LinearArgs& a, bool gradient) {
     const double out = (double)a.q_rows * a.p_cols * 4;
     for (long splits = 1; splits <= (gradient ? MAX_SPLITS : 1); splits += splits < 4 ? 1 : splits < 8 ? 2 : 4) {
         if (splits > 1 && (steps_of(a) < splits * MIN_STEPS || out * splits > split_bytes(a))) break;
-        const double sum = splits > 1 ? 4.5 + (2 * splits + 0.5) * out / 9e6 : 0.0;  // written and read, mostly in cache
+        const double sum = splits > 1 ? 3.7 + (2 * splits + 0.5) * out / 9.9e6 : 0.0;  // written and read, mostly in cache
         for (int kernel = 0; kernel < KERNELS; ++kernel) {
             // no room there for e4m3 fragments widened to bf16; Tall gains nothing by columns (9482 x 768
             // x 2304: 38.2 us, Pair 37.5)

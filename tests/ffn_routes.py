@@ -25,15 +25,15 @@ ROUTES = {
         "wide+deep": (2579, 3320, 416), "wide+pair": (4384, 4600, 432), "wide+tall": (11654, 1664, 784),
         "wide+wide": (1240, 8520, 5600)},
     ("dx", "half"): {
-        "small": (44, 152, 48), "small/parts": (40, 1080, 56), "deep": (16387, 152, 80), "deep/parts": (65, 3432, 3056),
-        "pair": (34480, 168, 56), "pair/parts": (2924, 4088, 80), "wide": (32894, 168, 168),
-        "wide/parts": (150, 5112, 5872), "wide+small": (17041, 152, 976), "wide+deep": (39191, 504, 400),
-        "wide+pair": (2570, 552, 8288)},
+        "small": (44, 152, 48), "small/parts": (40, 1080, 56), "deep": (17573, 200, 80), "deep/parts": (65, 3432, 3056),
+        "pair": (34480, 168, 56), "pair/parts": (67, 2520, 5856), "wide": (32894, 168, 168),
+        "wide/parts": (141, 8872, 2944), "wide+small": (17041, 152, 976), "wide+deep": (20115, 392, 800),
+        "wide+pair": (2699, 424, 7552), "wide+wide": (2710, 5512, 8288)},
     ("dw", "half"): {
-        "small": (151, 40, 48), "small/parts": (979, 40, 48), "deep": (151, 264, 6544), "deep/parts": (6742, 1368, 80),
+        "small": (151, 40, 48), "small/parts": (979, 40, 48), "deep": (151, 264, 6544), "deep/parts": (7176, 72, 1360),
         "pair": (154, 8816, 400), "pair/parts": (4035, 2752, 80), "wide": (161, 5992, 1344),
-        "wide/parts": (11370, 2720, 144), "wide+small": (153, 2088, 8176), "wide+deep": (502, 3608, 5040),
-        "wide+pair": (597, 3480, 6112), "wide+wide": (20156, 2832, 8256)},
+        "wide/parts": (6061, 136, 5680), "wide+small": (153, 2088, 8176), "wide+deep": (464, 6088, 2832),
+        "wide+pair": (530, 2864, 7280), "wide+wide": (8843, 5552, 7344)},
 }
 
 
