@@ -550,11 +550,16 @@ def linear_backward_workspace(rows, n, k, act="none") -> int:
 def linear_plan(product, dtype, rows, n, k, out_dtype=None):
     """jh_op_linear_plan: [(kernel, parts, rows)] of the one or two launches of a product ("linear", "gated", "dx" or
     "dw") of torch types; out_dtype is dtype (bfloat16 for e4m3) unless given."""
-    codes = _dtype_codes()
+    products, codes = ("linear", "gated", "dx", "dw"), _dtype_codes()
+    if product not in products:
+        _invalid(f"unknown product {product!r}")
+    for d in (dtype, out_dtype):
+        if d is not None and d not in codes:
+            _invalid(f"no such element type: {d}")
     t = codes[dtype]
     out = codes[out_dtype] if out_dtype is not None else abi.BF16 if t == abi.E4M3 else t
     launches = (LinearLaunch * 2)()
-    check(lib().jh_op_linear_plan(("linear", "gated", "dx", "dw").index(product), t, out, rows, n, k, launches))
+    check(lib().jh_op_linear_plan(products.index(product), t, out, rows, n, k, launches))
     names = ("small", "deep", "pair", "tall", "wide", "stream")
     return [(names[v.kernel], v.parts, v.rows) for v in launches if v.parts]
 

@@ -82,6 +82,14 @@ def test_plan_refusals(change):
     assert hip.lib().jh_op_linear_plan(*{**base, **change}.values()) == abi.JH_ERR_INVALID
 
 
+@pytest.mark.parametrize("args", [("dy", BF16, 8, 8, 8), ("linear", torch.int8, 8, 8, 8), ("linear", BF16, 8, 8, 8, torch.int8),
+                                  ("linear", BF16, 8, 12, 8), ("dw", E4M3, 16, 16, 16)])
+def test_plan_refusals_in_python(args):
+    with pytest.raises(hip.HipError) as e:
+        hip.linear_plan(*args)
+    assert e.value.code == abi.JH_ERR_INVALID
+
+
 @pytest.mark.parametrize("n,k", [(1024, 1024), (1024, 4096), (4096, 1024), (2304, 768), (4096, 4096), (264, 5000)])
 def test_a_contraction_is_planned_by_its_steps(n, k):
     """dw's contraction runs in steps of 64 rows, whose number decides the kernel and the parts; no other border does."""
