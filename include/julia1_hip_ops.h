@@ -264,7 +264,8 @@ enum {
  * (8 + E) 2^-23 of their value, E = z^2 and |z| (the tanh form: 4 times the argument
  * of its exponential), down to 2^-119.  A row's bits may depend
  * on the number of rows in the call (kernels are chosen by size).  Squares are
- * summed as they are: rows whose sum of squares passes 3.4e38 are not normalised.
+ * summed as they are: rows whose sum of squares passes 3.4e38 are not normalised, nor,
+ * with eps = 0, rows whose squares vanish in FP32.
  */
 
 /*

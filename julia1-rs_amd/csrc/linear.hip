@@ -49,8 +49,10 @@ __device__ inline void load8_of(const void* p, float (&v)[8]) {
 // dz = dy act'(pre) (rounded to T) and the column sums of its unrounded values, a part per
 // blockIdx.y.  A lane owns 8 columns, the four waves of a workgroup every fourth of its rows;
 // their sums are joined in wave order.  dz is kept because both products read it, one of them by
-// columns.  Bound by memory: 9482 x 1024 bf16 gelu, 58 MB, takes 18 to 20 us (3.1 TB/s; 3 more with four rows
-// in flight per wave).
+// columns, and rounded because the matrix instruction takes 16 bits: dx and dw are off by 0.0023
+// of their norm so (9482 x 1024 x 4096 bf16, against 64 bits), by 0.0017 for their own rounding
+// alone.  Bound by memory: 9482 x 1024 bf16 gelu, 58 MB, takes 18 to 20 us (3.1 TB/s; 3 more
+// with four rows in flight per wave).
 template <class T>
 __global__ __launch_bounds__(THREADS) void act_grad_kernel(ActGradArgs a) {
     __shared__ float join[4][64][9];
@@ -88,7 +90,7 @@ __global__ __launch_bounds__(THREADS) void act_grad_kernel(ActGradArgs a) {
     }
 }
 
-// [dg du] = [dh u act'(g), dh act(g)], rounded to T.  Bound by memory: 9482 x 1152 bf16, 109 MB,
+// [dg du] = [dh u act'(g), dh act(g)], rounded to T as dz is.  Bound by memory: 9482 x 1152 bf16, 109 MB,
 // takes 20 us (5.5 TB/s).
 template <class T>
 __global__ __launch_bounds__(THREADS) void gated_grad_kernel(GatedGradArgs a) {
@@ -112,7 +114,7 @@ __global__ __launch_bounds__(THREADS) void gated_grad_kernel(GatedGradArgs a) {
 }
 
 // out[r, c] = sum over s of partial[s][r, c], in split order.  Bound by memory: four parts of
-// 2304 x 768, 32 MB, take 6.2 us (5.1 TB/s).
+// 2304 x 768, 32 MB, take 6.2 us (5.1 TB/s), eight, 60 MB, 10 us (6 TB/s, partly from cache).
 template <class T>
 __global__ __launch_bounds__(THREADS) void split_sum_kernel(const float* partial, int splits, int rows, int cols,
                                                             void* out, long ldo, int out_f32) {

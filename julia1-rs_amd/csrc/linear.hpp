@@ -308,7 +308,7 @@ __device__ inline void store16(void* dst, const float (&v)[N]) {
 // lane % 16, four lanes 64 columns of it.  Lanes exchange 16-byte runs so that an instruction
 // covers whole 128-byte lines: 8 rows of 128 bytes in 16 bits, 4 rows of 256 in FP32.  (16 rows
 // of 64 bytes or of every other run keep the memory path busy for longer: 16384 x 4096 x 512 bf16
-// took 98.5 us so and takes 84.8, the FP32 parts of dw of 9482 x 2304 x 768 51.6 and 48.1.)  The
+// took 98.5 us so and takes 92, four FP32 parts of dw of 9482 x 2304 x 768 on 128 x 128 tiles 51.6 and 48.1.)  The
 // exchange is its own inverse: residuals are loaded in whole lines as well.
 //
 // Lane bit 3 (2) changes places with which of two runs it is.

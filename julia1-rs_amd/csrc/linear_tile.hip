@@ -14,7 +14,7 @@
 //          Pair's operand bytes
 //
 // Where each is taken, and what it measured, stands at cost() in linear.hip.  At their best, bf16:
-// Tall 1.15 PFLOP/s (2048 x 4096 x 4096), Pair 0.90 (dx of 9482 x 2304 x 768; MFMA busy 25 % of the
+// Tall 1.15 PFLOP/s (2048 x 4096 x 4096), Pair 0.90 (dx of 9482 x 2304 x 768; MFMA busy 27 % of the
 // time), Deep 0.60 (1024 x 4096 x 1024).  What bounds them is neither LDS (a quarter of its cycles
 // at most, no bank conflicts) nor the way from L2 (32 KB to a CU take 0.25 to 0.32 us with all CUs
 // reading, against 0.54 us for a step of Deep's), which leaves the step's barrier: a wave's MFMAs

@@ -5,7 +5,7 @@
 // Measured (MFMA busy and clock from counters): 16384 x 8192 x 2048 bf16 gated with silu and both
 // projections kept, 1.10 PFLOP in 891 us (1.23 PFLOP/s, busy 59 % at 1.91 GHz: power holds the
 // clock there, 2.4 GHz at rest); 8192 x 4096 x 4096 bf16 200 us (1.37); 4096^3 e4m3 57 us (2.40);
-// 8192 x 4096 x 4096 e4m3 105 us (2.6), with bias, silu and residual 125 (2.2): all tiles of a
+// 8192 x 4096 x 4096 e4m3 105 us (2.6), with bias, silu and residual 122 to 128 (2.2): all tiles of a
 // round end together, 67 MB of residuals and outputs in a burst, twice.  LDS is read a fifth of
 // the time, without bank conflicts; a step's 64 KB of operands take half as long to come in as its
 // MFMAs (2048 cycles), all CUs reading.
@@ -28,8 +28,8 @@
 //
 // LDS holds two K steps of four 16 KB parts, two of either operand.  Q's hold its first and last
 // 128 rows (columns, where k is the row index), 32 of each for a wave.  P's: by columns the first
-// and last 128, 64 of each for a wave (one run of 256 bytes per k; the weight gradient of 29367 x
-// 3464 x 1504 took 403 us so, 426 in runs of 64 and 128); by rows the first and last 64 of a
+// and last 128, 64 of each for a wave (one run of 256 bytes per k; when this was chosen the weight
+// gradient of 29367 x 3464 x 1504, now 283 us in parts, took 403 so and 426 in runs of 64 and 128); by rows the first and last 64 of a
 // wave's 128 (16384 x 4096 x 512: 91 us, 94 with the halves 128 apart); gated the gate's 128 rows
 // and the up projection's.  So a lane ends with 16 consecutive output columns and four lanes with
 // 64 of a row, whatever the layout: the epilogue writes whole 128-byte lines.  A part read in
