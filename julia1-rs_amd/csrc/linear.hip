@@ -3,7 +3,6 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <cmath>
 
 #include "linear.hpp"
 
@@ -170,12 +169,12 @@ long tiles_of(const LinearArgs& a, int p, int q) {
 // What a launch of each kernel takes, in us, from its number of tiles and of K steps: a start
 // and an end per round of tiles (launch, first loads, epilogue) and a time per step that grows
 // with the CUs at work (shared L2 and power).  The constants are fits to times on an MI355X (256 CUs):
-// products to 86 sizes whose inputs, in three sets, take turns, as a layer meets its own (of 633
-// ways to run them the kernel that comes out cheapest takes 0.3 % longer than the fastest in the
-// mean, 11 % at worst); gradients to 124 sizes, log-uniform ones and training widths, with as many
-// sets of inputs as 700 MB hold, so that none is left in the 256 MB of cache, but dz just written, as the
-// activation's gradient leaves it (0.6 % and 11 %; on 140 other sizes 1.1 % and 18 %).  Some of them,
-// bf16, gradients in their best number of parts (us, the kernel taken in brackets):
+// forward products to 42 sizes whose inputs, in three sets, take turns, as a layer meets its own (the
+// kernel that comes out cheapest takes 0.1 % longer than the fastest in the mean, 6 % at worst);
+// gradients to 124 sizes, log-uniform ones and training widths, with as many sets of inputs as 700 MB
+// hold, so that none is left in the 256 MB of cache, but dz just written, as the activation's gradient
+// leaves it (0.6 % and 11 %; on 140 other sizes 1.1 % and 18 %).  Some of them, bf16, gradients in
+// their best number of parts (us, the kernel taken in brackets):
 //
 //   rows x n x k              Small   Deep    Pair    Tall    256 x 256
 //   512 x 768 x 768           [7.0]   9.9     12.2    13.8    21.2
