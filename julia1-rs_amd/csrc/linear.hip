@@ -170,7 +170,8 @@ long tiles_of(const LinearArgs& a, int p, int q) {
 // and an end per round of tiles (launch, first loads, epilogue) and a time per step that grows
 // with the CUs at work (shared L2 and power).  The constants are fits to times on an MI355X (256 CUs):
 // forward products to 42 sizes whose inputs, in three sets, take turns, as a layer meets its own (the
-// kernel that comes out cheapest takes 0.1 % longer than the fastest in the mean, 6 % at worst);
+// kernel that comes out cheapest takes 0.1 % longer than the fastest in the mean, 6 % at worst; on 110
+// other sizes, inputs out of cache and whole rounds of 256 x 256 tiles among the choices, 1.7 % and 25 %);
 // gradients to 124 sizes, log-uniform ones and training widths, with as many sets of inputs as 700 MB
 // hold, so that none is left in the 256 MB of cache, but dz just written, as the activation's gradient
 // leaves it (0.6 % and 11 %; on 140 other sizes 1.1 % and 18 %).  Some of them, bf16, gradients in
